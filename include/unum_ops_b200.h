@@ -373,6 +373,69 @@ int unum_compress_keys(const void *k, int64_t T, int64_t Hk, int64_t D, int64_t 
                        const int32_t *cu_seqlens, const int32_t *cu_out, int64_t n_seq, int64_t n_out,
                        int64_t kernel, int64_t stride, void *out, void *stream);
 
+/*
+ * The paged key-value cache: caches [n_tokens, Hk, D] of bf16 or fp16 (D = 64 or 128; strides in elements,
+ * multiples of 8; 16-byte aligned), and a table [B, n_pages] (row stride bt_stride) that puts position p of
+ * sequence b at token  table[b, p / page_size] * page_size + p % page_size;  page_size is a power of two up to
+ * 65536, and 1 is the table that unum_get_block_table reads.  A table entry whose token is outside
+ * [0, n_tokens) marks positions that are not held.  No reference functions: the reference leaves the cache and
+ * dense attention over it to its caller (get_table_torch.py:29-44 fixes the mapping).
+ */
+
+/*
+ * cache_append — writes new tokens' keys and values to their places.
+ *   k, v     [T, Hk, D] of the cache's 2-byte type (strides in elements, multiples of 8; 16-byte aligned)
+ *   token_to_bs, token_pos_in_bs  int32 [T]: token t is position token_pos_in_bs[t] - 1 of its sequence (the last
+ *            of the positions it sees, as for unum_get_block_table)
+ * A token whose sequence is outside [0, B), whose position is outside the table or whose table entry is not held
+ * is not written; rows that no token goes to are left as they were.  Places must differ from token to token.
+ */
+int unum_cache_append(const void *k, const void *v, int64_t T, int64_t Hk, int64_t D, int64_t k_st, int64_t k_sh,
+                      int64_t v_st, int64_t v_sh, void *k_cache, void *v_cache, int64_t n_tokens, int64_t kc_st,
+                      int64_t kc_sh, int64_t vc_st, int64_t vc_sh, const int32_t *block_table, int64_t B,
+                      int64_t n_pages, int64_t bt_stride, int64_t page_size, const int32_t *token_to_bs,
+                      const int32_t *token_pos_in_bs, void *stream);
+
+/*
+ * paged_attention — attention of one new token for each sequence over its cache.
+ *   q        dtype [B, Hq, D] (UNUM_DTYPE_BF16 or UNUM_DTYPE_F16, the cache's type), Hq = G * Hk, G <= 64
+ *   seqlens  int32 [B]: positions [0, seqlens[b]) are attended to (clamped to [0, max_seqlen])
+ *   max_seqlen <= n_pages * page_size
+ *   out      dtype [B, Hq, D] contiguous, fully written;  lse  float [B, Hq] or NULL
+ *   weights  float [B, Hk, >= max_seqlen] or NULL (strides w_sb, w_sh): updated in place
+ *   workspace  unum_paged_attention_workspace_size(...) bytes, 16-byte aligned, any contents, not shared with a
+ *            call that may run at the same time
+ *
+ *   s[p] = softmax_scale * q[b,h] . k[token(p), g],  g = h / G;   lse[b,h] = log sum_p exp(s[p])
+ *   out[b,h] = sum_p exp(s[p] - lse) v[token(p), g];   weights[b,g,p] += sum_{h in group g} exp(s[p] - lse)
+ * over the held positions; a row with none (or only scores of -inf) is 0 with lse = -inf.
+ */
+size_t unum_paged_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t max_seqlen,
+                                           int gather_weights);
+int unum_paged_attention(const void *q, int64_t B, int64_t Hq, int64_t D, int64_t q_sb, int64_t q_sh,
+                         const void *k_cache, const void *v_cache, int dtype, int64_t n_tokens, int64_t Hk,
+                         int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh, const int32_t *block_table,
+                         int64_t n_pages, int64_t bt_stride, int64_t page_size, const int32_t *seqlens,
+                         int64_t max_seqlen, float softmax_scale, void *out, float *lse, float *weights,
+                         int64_t w_sb, int64_t w_sh, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * cache_evict — shortens each sequence's cache to `budget` pages by the attention weight that its positions gathered.
+ *   weights  float [B, Hk, n_pages * page_size] (strides w_sb, w_sh; positions contiguous)
+ * Of the pages in use the first init_pages, the last local_pages (>= 1) and the heaviest others stay, `budget` in
+ * all, in their order.  A page's weight is the sum over kv heads and the page's positions, in 64 bits and rounded
+ * to 32 once; ties stay by the lower index, a NaN ranks below every number.  All outputs are fully written:
+ *   new_table   int32 [B, n_pages]: the row without the evicted entries, then -1
+ *   new_seqlens int32 [B]: less page_size for each evicted page
+ *   new_weights float [B, Hk, n_pages * page_size]: moved along with their pages, 0 behind the new length
+ *   evicted     int32 [B, n_pages]: the evicted entries in their order, then -1
+ * The outputs must not overlap the inputs.  n_pages <= 409600 and n_pages * page_size < 2^31.
+ */
+int unum_cache_evict(const int32_t *block_table, int64_t B, int64_t n_pages, int64_t bt_stride,
+                     const int32_t *seqlens, const float *weights, int64_t Hk, int64_t w_sb, int64_t w_sh,
+                     int64_t page_size, int64_t budget, int64_t init_pages, int64_t local_pages, int32_t *new_table,
+                     int32_t *new_seqlens, float *new_weights, int32_t *evicted, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

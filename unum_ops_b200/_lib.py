@@ -60,6 +60,14 @@ SIGNATURES = {
     "unum_sparse_attn_blocks": ([_p, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _i64,
                                  _p, _i64, _i64, _i64, _p, _p, _int, _p, _int, _i32, ctypes.c_float, _p,
                                  _p, _p], _int),
+    "unum_cache_append": ([_p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64,
+                           _p, _i64, _i64, _i64, _i64, _p, _p, _p], _int),
+    "unum_paged_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _int], ctypes.c_size_t),
+    "unum_paged_attention": ([_p, _i64, _i64, _i64, _i64, _i64, _p, _p, _int, _i64, _i64, _i64, _i64, _i64, _i64, _p,
+                              _i64, _i64, _i64, _p, _i64, ctypes.c_float, _p, _p, _p, _i64, _i64, _p,
+                              ctypes.c_size_t, _p], _int),
+    "unum_cache_evict": ([_p, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p],
+                         _int),
     "unum_infllmv2_attn_stage1_noalloc": ([_p, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64,
                                            _i64, _p, _p, _i64, ctypes.c_float, _int, _p, _i64, _p],
                                           _int),
