@@ -79,7 +79,7 @@ def oracle_evict(table, lens, w, budget, init, local, page):
         rank = sorted(range(used), key=lambda e: (not (e < init or e >= used - local), bool(np.isnan(score[e])),
                                                   0.0 if np.isnan(score[e]) else -score[e], e))
         keep = sorted(rank[:budget]) if used > budget else list(range(used))
-        out = [e for e in range(used) if e not in set(keep)]
+        out = sorted(set(range(used)) - set(keep))
         row = keep + list(range(used, n_pages))
         new_table[b, :len(row)] = table[b, row]
         gone[b, :len(out)] = table[b, out]

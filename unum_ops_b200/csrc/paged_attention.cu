@@ -7,6 +7,25 @@
 //     s_p = scale * q[b,h] . k[token(p), g];   lse = log sum_p exp(s_p);   out = sum_p exp(s_p - lse) v[token(p), g]
 //     weights[b,g,p] += sum over the group's heads of exp(s_p - lse)          (where they are gathered)
 // A row without a valid position is 0 with lse = -inf.
+//
+// What bounds it: each key and value row is read once, 4 * D bytes a position and kv head, against 4 * D * G operations:
+// at G = 16 and HBM's full rate 100 TFLOP/s, 6% of the tensor cores.  So everything serves the loads:
+//   - work is split over the length in units of 64 positions.  The units of all (sequence, kv head) items, in a row,
+//     are dealt to the resident blocks in equal shares (two blocks an SM, one wave), so a batch of any lengths, one
+//     long sequence or many short ones, loads every SM alike;
+//   - a block's four warps take 16 positions of a unit each.  A warp (a team of 2 or 4 warps where G > 16: one for
+//     each 16 heads) has a ring of its own in shared memory, filled by 16-byte asynchronous copies that gather rows by
+//     the table, whose entries are read one step ahead.  No block-wide barrier is in the loop, and the copies run on
+//     across items;
+//   - the products are m16n8k16 matrix instructions with the 16 heads as rows: scores and probabilities stay in
+//     registers (the scores' layout is the layout that the second product wants), the softmax's running maximum and
+//     sum in 32 bits; the output accumulates in registers and is rescaled only where a maximum moved;
+//   - where an item is cut, each block leaves its maximum, sum and output in the workspace and the second kernel joins
+//     them in the order of the positions (the same bits each time).  It is launched early (programmatic dependent
+//     launch) and waits for the first.  It also turns the scores, left in the workspace in 32 bits, into weights: their
+//     sum over the group needs each head's final lse, and reading 4 * G bytes back costs less than the key again.
+// Roundings: the probabilities go to the cache's type for the product with v (the sum l uses them unrounded), and the
+// output once at the end.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -14,133 +33,623 @@
 
 namespace {
 
-constexpr int kTile = 32;
-constexpr int kThreads = 256;
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kBlocksPerSm = 2;
+constexpr int kUnit = 64;            // positions dealt to a block at a time
+constexpr int kStep = 16;            // positions of a team's step: a unit is kWarps steps of 16
+constexpr int kGrain = 2;            // units a block takes at least: below it the join costs more than the split gains
+constexpr int kMaxWorkers = 512;     // resident blocks, at most
+constexpr uint32_t kRingBytes = 96 * 1024;
 constexpr int kMaxG = 64;
+constexpr int kJoinThreads = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct Params {
-    const void *q, *kc, *vc;
-    int64_t q_sb, q_sh, k_st, k_sh, v_st, v_sh;
+    const uint8_t *q, *kc, *vc;
+    int64_t q_sb, q_sh, k_st, k_sh, v_st, v_sh;  // bytes
     const int32_t *table, *lens;
-    int64_t bt_stride, n_tokens, max_len;
-    int32_t shift, Hk, G;
+    int64_t bt_stride, n_tokens;
+    int32_t max_len, shift, B, Hk, G, workers;
     float c;  // scale * log2(e)
     void *out;
     float *lse, *weights;
     int64_t w_sb, w_sh;
+    // workspace
+    int2 *span;          // [B * Hk]: first and last block of the item
+    float *lse2;         // [B * Hk][16 * MT]: of items that one block holds, in base 2
+    float2 *part_ml;     // [2 * workers][16 * MT]: maximum (base 2) and sum
+    float4 *part_o;      // [2 * workers][MT][D / 8][32 lanes]
+    float *scores;       // [B * Hk][G][score_ld], base 2
+    int64_t score_ld;
 };
 
-template <typename T> __device__ __forceinline__ float to_f(T x);
-template <> __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <> __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-template <typename T> __device__ __forceinline__ T from_f(float x);
-template <> __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
-template <> __device__ __forceinline__ __half from_f(float x) { return __float2half_rn(x); }
+// ---------------------------------------------------------------------------------------------- instructions
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
-// The simplest right form: one block for each (sequence, kv head), products on the CUDA cores.
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant__ Params p) {
-    extern __shared__ float sm[];
-    const int G = p.G;
-    float *q = sm, *o = q + G * D, *kv = o + G * D, *s = kv + kTile * (D + 1), *m = s + G * kTile, *l = m + G, *f = l + G;
-    __shared__ int64_t tok[kTile];
-    const int g = blockIdx.x, tid = threadIdx.x;
-    const int64_t b = blockIdx.y;
-    const T *qp = (const T *)p.q, *kc = (const T *)p.kc + g * p.k_sh, *vc = (const T *)p.vc + g * p.v_sh;
-    int64_t len = p.lens[b];
-    len = len < 0 ? 0 : (len > p.max_len ? p.max_len : len);
-    for (int i = tid; i < G * D; i += kThreads) {
-        q[i] = to_f(qp[b * p.q_sb + (int64_t)(g * G + i / D) * p.q_sh + i % D]);
-        o[i] = 0.f;
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T> struct Num;
+template <> struct Num<__nv_bfloat16> {
+    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
-    for (int i = tid; i < G; i += kThreads) m[i] = -INFINITY, l[i] = 0.f;
-    auto load = [&](const T *c, int64_t st) {
-        for (int i = tid; i < kTile * D; i += kThreads) {
-            const int64_t t = tok[i / D];
-            kv[i / D * (D + 1) + i % D] = t >= 0 ? to_f(c[t * st + i % D]) : 0.f;
+    static __device__ __forceinline__ uint32_t pack(float x, float y) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+};
+template <> struct Num<__half> {
+    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+    static __device__ __forceinline__ uint32_t pack(float x, float y) {
+        const __half2 v = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+};
+
+// ---------------------------------------------------------------------------------------------- the order of the work
+__device__ __forceinline__ int32_t length(const Params &p, int32_t b) {
+    const int32_t n = __ldg(p.lens + b);
+    return n < 0 ? 0 : (n > p.max_len ? p.max_len : n);
+}
+__device__ __forceinline__ int32_t units_of(int32_t len) { return (len + kUnit - 1) / kUnit; }
+
+// A place in the row of units: sequence, kv head, unit of the item.
+struct Place {
+    int32_t b, h, unit, units, len;
+    __device__ __forceinline__ void set(const Params &p, int32_t b_) {
+        b = b_;
+        len = b < p.B ? length(p, b) : 0;
+        units = units_of(len);
+    }
+    __device__ __forceinline__ void next_item(const Params &p) {
+        unit = 0;
+        if (++h < p.Hk) return;
+        h = 0;
+        do set(p, b + 1);
+        while (units == 0 && b < p.B);
+    }
+    __device__ __forceinline__ void next(const Params &p) {
+        if (++unit == units) next_item(p);
+    }
+};
+
+// Units before this thread's share of the sequences, and the total (over one kv head).  All threads call it.
+template <int kN>
+__device__ __forceinline__ int64_t scan_units(const Params &p, int32_t b0, int32_t b1, int64_t *warp_sums, int64_t &total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t mine = 0;
+    for (int32_t b = b0; b < b1; ++b) mine += units_of(length(p, b));
+    int64_t x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sums[warp] = x;
+    __syncthreads();
+    int64_t before = x - mine;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kN; ++w) {
+        if (w < warp) before += warp_sums[w];
+        total += warp_sums[w];
+    }
+    return before;
+}
+
+template <int MT> __device__ __forceinline__ void team_sync(int team) {
+    if (MT == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(MT * 32) : "memory");
+}
+
+// MT = 16-head tiles of a group (1, 2 or 4): the warps of a team.
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __grid_constant__ Params p) {
+    constexpr int kTeams = kWarps / MT;
+    constexpr int kRow = D * 2;                          // bytes
+    constexpr uint32_t kHalf = kStep * kRow, kSlot = 2 * kHalf;  // keys, values of a step
+    constexpr int kSlots = kRingBytes / (kTeams * kSlot) > 8 ? 8 : kRingBytes / (kTeams * kSlot);
+    constexpr int kLanes = kRow / 16, kRows = 32 / kLanes;  // lanes of a row, rows of one copy instruction
+    constexpr int kCopies = kStep / kRows / MT;             // of each warp, for keys and for values
+    static_assert(kCopies >= 1 && kSlots >= 3, "a step must give every warp a copy");
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ uint32_t held[kTeams][8];                 // which of a slot's positions are valid
+    __shared__ int64_t warp_sums[kWarps];
+    __shared__ int32_t start[3];
+    __shared__ float2 merge_ml[2][16 * 2];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, team = warp / MT, ht = warp % MT;
+    const uint32_t ring = smem_u32(smem) + team * (kSlots * kSlot);
+    float4 *merge = reinterpret_cast<float4 *>(smem + kTeams * kSlots * kSlot);  // [2][D / 8][32]
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // this block's share of the units
+    const int32_t per = (p.B + kThreads - 1) / kThreads;
+    const int32_t b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
+    int64_t total, before = scan_units<kWarps>(p, b0, b1, warp_sums, total);
+    before *= p.Hk;
+    total *= p.Hk;
+    int64_t workers = (total + kGrain - 1) / kGrain;
+    if (workers > p.workers) workers = p.workers;
+    const int64_t me = blockIdx.x;
+    if (me >= workers) return;
+    const int64_t u0 = me * total / workers, u1 = (me + 1) * total / workers;
+    for (int32_t b = b0; b < b1; ++b) {
+        const int32_t n = units_of(length(p, b));
+        const int64_t mine = (int64_t)n * p.Hk;
+        if (u0 >= before && u0 < before + mine) {
+            const int64_t r = u0 - before;
+            start[0] = b;
+            start[1] = (int32_t)(r / n);
+            start[2] = (int32_t)(r % n);
+        }
+        before += mine;
+    }
+    __syncthreads();
+    Place in;  // where the loads are
+    in.set(p, start[0]);
+    in.h = start[1];
+    in.unit = start[2];
+    Place at = in;  // where the arithmetic is
+    const int64_t steps = (u1 - u0) * MT;
+    int64_t fetched = 0;
+    int in_k = 0;
+
+    // the next step's token of position lane % 16 (or -1), read ahead of its copies
+    int32_t tok = -1, tok_h = 0;
+    auto fetch = [&]() {
+        tok = -1;
+        if (fetched >= steps) return;
+        const int32_t pos = in.unit * kUnit + (team + kTeams * in_k) * kStep + (lane & 15);
+        tok_h = in.h;
+        if (pos < in.len) {
+            const int64_t page = __ldg(p.table + in.b * p.bt_stride + (pos >> p.shift));
+            const int64_t t = (page << p.shift) + (pos & ((1 << p.shift) - 1));
+            tok = page >= 0 && t < p.n_tokens ? (int32_t)t : -1;
+        }
+        ++fetched;
+        if (++in_k == MT) {
+            in_k = 0;
+            in.next(p);
         }
     };
-    auto scores = [&](int64_t p0) {
-        __syncthreads();
-        if (tid < kTile) {
-            const int64_t at = p0 + tid;
-            int64_t t = -1;
-            if (at < len) {
-                const int64_t page = p.table[b * p.bt_stride + (at >> p.shift)];
-                t = (page << p.shift) + (at & ((1 << p.shift) - 1));
-                if (page < 0 || t >= p.n_tokens) t = -1;
+    // its copies into a slot
+    auto issue = [&](uint32_t slot) {
+        const uint32_t mask = __ballot_sync(0xffffffffu, tok >= 0) & 0xffffu;
+        if (ht == 0 && lane == 0) held[team][slot] = mask;
+        if (mask) {
+            const uint8_t *kb = p.kc + (int64_t)tok_h * p.k_sh + (lane % kLanes) * 16;
+            const uint8_t *vb = p.vc + (int64_t)tok_h * p.v_sh + (lane % kLanes) * 16;
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) {
+                const int row = (i * MT + ht) * kRows + lane / kLanes;
+                const int32_t t = __shfl_sync(0xffffffffu, tok, row);
+                const uint32_t dst = ring + slot * kSlot + row * kRow + (((lane % kLanes) ^ (row & 7)) << 4);
+                const int64_t o = t < 0 ? 0 : t;
+                cp_async16(dst, kb + o * p.k_st, t < 0 ? 0u : 16u);
+                cp_async16(dst + kHalf, vb + o * p.v_st, t < 0 ? 0u : 16u);
             }
-            tok[tid] = t;
         }
-        __syncthreads();
-        load(kc, p.k_st);
-        __syncthreads();
-        for (int i = tid; i < G * kTile; i += kThreads) {
-            const int h = i / kTile, j = i % kTile;
-            float x = 0.f;
-            for (int d = 0; d < D; ++d) x = fmaf(q[h * D + d], kv[j * (D + 1) + d], x);
-            s[i] = tok[j] >= 0 ? x * p.c : -INFINITY;
-        }
-        __syncthreads();
+        cp_commit();
+        fetch();
     };
-    for (int64_t p0 = 0; p0 < len; p0 += kTile) {
-        scores(p0);
-        for (int h = tid; h < G; h += kThreads) {
-            float mx = m[h];
-            for (int j = 0; j < kTile; ++j) mx = fmaxf(mx, s[h * kTile + j]);
-            const float base = mx == -INFINITY ? 0.f : mx;
-            float sum = 0.f;
-            for (int j = 0; j < kTile; ++j) {
-                const float e = exp2f(s[h * kTile + j] - base);
-                s[h * kTile + j] = e;
-                sum += e;
+
+    fetch();
+#pragma unroll 1
+    for (int s = 0; s < kSlots - 1; ++s) issue(s);
+
+    uint32_t slot = 0;
+    const int r0 = lane >> 2, c0 = (lane & 3) * 2;
+    int64_t u = u0;
+    while (u < u1) {
+        // one item's units in this block
+        const int64_t seg_end = min(u + (at.units - at.unit), u1);
+        const bool from_start = at.unit == 0, to_end = u + (at.units - at.unit) == seg_end;
+        const int64_t item = (int64_t)at.b * p.Hk + at.h;
+        const int64_t item_u0 = u - at.unit;
+        uint32_t qa[D / 16][4];
+        {
+            const uint8_t *qb = p.q + at.b * p.q_sb + (int64_t)(at.h * p.G + ht * 16) * p.q_sh + c0 * 2;
+            const int left = p.G - ht * 16;
+            const uint8_t *q0 = qb + r0 * p.q_sh, *q1 = qb + (r0 + 8) * p.q_sh;
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+                qa[k][0] = r0 < left ? __ldg(reinterpret_cast<const uint32_t *>(q0 + k * 32)) : 0u;
+                qa[k][1] = r0 + 8 < left ? __ldg(reinterpret_cast<const uint32_t *>(q1 + k * 32)) : 0u;
+                qa[k][2] = r0 < left ? __ldg(reinterpret_cast<const uint32_t *>(q0 + k * 32 + 16)) : 0u;
+                qa[k][3] = r0 + 8 < left ? __ldg(reinterpret_cast<const uint32_t *>(q1 + k * 32 + 16)) : 0u;
             }
-            f[h] = exp2f(m[h] - base);
-            l[h] = l[h] * f[h] + sum;
-            m[h] = mx;
         }
-        load(vc, p.v_st);
+        float o[D / 8][4];
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+        float *sc = p.scores + (item * p.G + ht * 16 + r0) * p.score_ld + c0;
+
+        for (; u < seg_end; ++u, ++at.unit) {
+#pragma unroll 1
+            for (int k = 0; k < MT; ++k) {
+                cp_wait<kSlots - 2>();
+                team_sync<MT>(team);  // the slot is filled, and nobody reads the one before it any more
+                issue(slot == 0 ? kSlots - 1 : slot - 1);
+                const uint32_t mask = held[team][slot];
+                const uint32_t kb = ring + slot * kSlot, vb = kb + kHalf;
+                slot = slot + 1 == kSlots ? 0 : slot + 1;
+                if (mask == 0 && !p.weights) continue;
+                float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+                if (mask) {
+                    const int row = (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        uint32_t f[4];
+                        ldsm4(f, kb + row * kRow + (((2 * kk + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
+                        Num<T>::mma(s[0], qa[kk], f[0], f[1]);
+                        Num<T>::mma(s[1], qa[kk], f[2], f[3]);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[t][e] = (mask >> (8 * t + c0 + (e & 1))) & 1u ? s[t][e] * p.c : -INFINITY;
+                if (p.weights) {
+                    const int64_t pos = (int64_t)at.unit * kUnit + (team + kTeams * k) * kStep;
+                    if (pos < at.len) {
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            if (ht * 16 + r0 < p.G)
+                                *reinterpret_cast<float2 *>(sc + pos + 8 * t) = make_float2(s[t][0], s[t][1]);
+                            if (ht * 16 + r0 + 8 < p.G)
+                                *reinterpret_cast<float2 *>(sc + 8 * p.score_ld + pos + 8 * t) =
+                                    make_float2(s[t][2], s[t][3]);
+                        }
+                    }
+                    if (mask == 0) continue;
+                }
+                float x0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+                float x1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+#pragma unroll
+                for (int i = 1; i <= 2; i <<= 1) {
+                    x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, i));
+                    x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, i));
+                }
+                if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
+                    x0 = fmaxf(x0, m0);
+                    x1 = fmaxf(x1, m1);
+                    const float a0 = x0 == -INFINITY ? 1.f : ex2(m0 - x0), a1 = x1 == -INFINITY ? 1.f : ex2(m1 - x1);
+                    m0 = x0;
+                    m1 = x1;
+                    l0 *= a0;
+                    l1 *= a1;
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i) {
+                        o[i][0] *= a0;
+                        o[i][1] *= a0;
+                        o[i][2] *= a1;
+                        o[i][3] *= a1;
+                    }
+                }
+                const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    s[t][0] = ex2(s[t][0] - z0);
+                    s[t][1] = ex2(s[t][1] - z0);
+                    s[t][2] = ex2(s[t][2] - z1);
+                    s[t][3] = ex2(s[t][3] - z1);
+                    l0 += s[t][0] + s[t][1];
+                    l1 += s[t][2] + s[t][3];
+                }
+                uint32_t a[4] = {Num<T>::pack(s[0][0], s[0][1]), Num<T>::pack(s[0][2], s[0][3]),
+                                 Num<T>::pack(s[1][0], s[1][1]), Num<T>::pack(s[1][2], s[1][3])};
+                const int row = lane & 15;
+#pragma unroll
+                for (int nn = 0; nn < D / 16; ++nn) {
+                    uint32_t f[4];
+                    ldsm4t(f, vb + row * kRow + (((2 * nn + (lane >> 4)) ^ (row & 7)) << 4));
+                    Num<T>::mma(o[2 * nn], a, f[0], f[1]);
+                    Num<T>::mma(o[2 * nn + 1], a, f[2], f[3]);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 1; i <= 2; i <<= 1) {
+            l0 += __shfl_xor_sync(0xffffffffu, l0, i);
+            l1 += __shfl_xor_sync(0xffffffffu, l1, i);
+        }
+        // the teams' parts, halving: the upper half leaves its own, the lower half takes it in
+#pragma unroll
+        for (int half = kTeams / 2; half >= 1; half >>= 1) {
+            const int spot = (team % half) * MT + ht;  // at most two
+            float4 *box = merge + spot * (D / 8) * 32 + lane;
+            if (team >= half && team < 2 * half) {
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) box[i * 32] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+                if ((lane & 3) == 0) {
+                    merge_ml[spot][r0] = make_float2(m0, l0);
+                    merge_ml[spot][r0 + 8] = make_float2(m1, l1);
+                }
+            }
+            __syncthreads();
+            if (team < half) {
+                const float2 y0 = merge_ml[spot][r0], y1 = merge_ml[spot][r0 + 8];
+                const float n0 = fmaxf(m0, y0.x), n1 = fmaxf(m1, y1.x);
+                const float z0 = n0 == -INFINITY ? 0.f : n0, z1 = n1 == -INFINITY ? 0.f : n1;
+                const float a0 = ex2(m0 - z0), a1 = ex2(m1 - z1), e0 = ex2(y0.x - z0), e1 = ex2(y1.x - z1);
+                m0 = n0;
+                m1 = n1;
+                l0 = l0 * a0 + y0.y * e0;
+                l1 = l1 * a1 + y1.y * e1;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    const float4 y = box[i * 32];
+                    o[i][0] = o[i][0] * a0 + y.x * e0;
+                    o[i][1] = o[i][1] * a0 + y.y * e0;
+                    o[i][2] = o[i][2] * a1 + y.z * e1;
+                    o[i][3] = o[i][3] * a1 + y.w * e1;
+                }
+            }
+            __syncthreads();
+        }
+        if (team == 0) {
+            if (from_start && to_end) {  // the whole item
+                const float i0 = l0 != 0.f ? 1.f / l0 : 0.f, i1 = l1 != 0.f ? 1.f / l1 : 0.f;
+                const float z0 = l0 != 0.f ? m0 + log2f(l0) : -INFINITY, z1 = l1 != 0.f ? m1 + log2f(l1) : -INFINITY;
+                const int left = p.G - ht * 16;
+                uint32_t *op = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p.out) +
+                                                            ((item * p.G + ht * 16 + r0) * D + c0) * 2);
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    if (r0 < left) op[i * 4] = Num<T>::pack(o[i][0] * i0, o[i][1] * i0);
+                    if (r0 + 8 < left) op[i * 4 + 4 * D] = Num<T>::pack(o[i][2] * i1, o[i][3] * i1);
+                }
+                if ((lane & 3) == 0) {
+                    float *z = p.lse2 + item * (16 * MT) + ht * 16 + r0;
+                    z[0] = z0;
+                    z[8] = z1;
+                    if (p.lse) {
+                        float *l = p.lse + item * p.G + ht * 16 + r0;
+                        if (r0 < left) l[0] = z0 * kLn2;
+                        if (r0 + 8 < left) l[8] = z1 * kLn2;
+                    }
+                }
+            } else {
+                // an item's first part is its block's last work, every other part its block's first
+                const int64_t spot = 2 * me + (from_start ? 1 : 0);
+                float4 *po = p.part_o + (spot * MT + ht) * (D / 8) * 32 + lane;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) po[i * 32] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+                if ((lane & 3) == 0) {
+                    float2 *ml = p.part_ml + spot * (16 * MT) + ht * 16 + r0;
+                    ml[0] = make_float2(m0, l0);
+                    ml[8] = make_float2(m1, l1);
+                }
+            }
+            if (to_end && warp == 0 && lane == 0) {
+                // the block with the item's first unit: the last one whose share begins at or before it
+                const int64_t first = ((item_u0 + 1) * workers - 1) / total;
+                p.span[item] = make_int2((int32_t)first, (int32_t)me);
+            }
+        }
+        at.unit = at.units - 1;
+        at.next(p);
+    }
+    cp_wait<0>();
+}
+
+// Joins the parts of items that were cut (blocks y < splits: each has 16 / slices of the output's 8-column tiles of one
+// 16-head tile, `slices` warps sharing a column's parts), and gathers weights (the others).  Blocks x: items.
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p, int32_t slices, int32_t splits) {
+    constexpr int kJoinWarps = kJoinThreads / 32;
+    __shared__ float factor[kMaxWorkers][16];  // of each part and head: 2^(m - M) / L
+    __shared__ float4 sums[kJoinWarps][32];
+    __shared__ float z[kMaxG];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int64_t item = blockIdx.x;
+    const int32_t b = (int32_t)(item / p.Hk), g = (int32_t)(item % p.Hk);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int32_t len = length(p, b);
+    const bool join = (int)blockIdx.y < splits;
+    if (len == 0) {
+        if (blockIdx.y == 0) {
+            uint32_t *op = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p.out) + item * p.G * D * 2);
+            for (int i = tid; i < p.G * D / 2; i += kJoinThreads) op[i] = 0u;
+            if (p.lse)
+                for (int i = tid; i < p.G; i += kJoinThreads) p.lse[item * p.G + i] = -INFINITY;
+        }
+        return;
+    }
+    const int2 sp = __ldcg(&p.span[item]);
+    const int32_t parts = sp.y - sp.x + 1;
+    if (join && parts == 1) return;
+    auto spot = [&](int32_t i) { return 2 * (int64_t)(sp.x + i) + (i == 0 ? 1 : 0); };
+    // M and L of each head: one warp a head
+    auto stats = [&](int ht, bool factors) {
+        const int64_t row = ht * 16 + warp;
+        float M = -INFINITY, L = 0.f;
+        for (int32_t i = lane; i < parts; i += 32) M = fmaxf(M, __ldcg(&p.part_ml[spot(i) * (16 * MT) + row]).x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        const float base = M == -INFINITY ? 0.f : M;
+        for (int32_t i = lane; i < parts; i += 32) {
+            const float2 v = __ldcg(&p.part_ml[spot(i) * (16 * MT) + row]);
+            L += v.y * ex2(v.x - base);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+        if (factors) {
+            const float inv = L != 0.f ? 1.f / L : 0.f;
+            for (int32_t i = lane; i < parts; i += 32)
+                factor[i][warp] = ex2(__ldcg(&p.part_ml[spot(i) * (16 * MT) + row]).x - base) * inv;
+        }
+        return L != 0.f ? M + log2f(L) : -INFINITY;
+    };
+    if (join) {
+        const int per = kJoinWarps / slices;              // 8-column tiles of this block
+        const int ht = blockIdx.y / (D / 8 / per), tile = blockIdx.y % (D / 8 / per) * per + warp / slices;
+        const float lse2 = stats(ht, true);
+        if (p.lse && blockIdx.y % (D / 8 / per) == 0 && lane == 0 && ht * 16 + warp < p.G)
+            p.lse[item * p.G + ht * 16 + warp] = lse2 * kLn2;
         __syncthreads();
-        for (int i = tid; i < G * D; i += kThreads) {
-            float x = o[i] * f[i / D];
-            for (int j = 0; j < kTile; ++j) x = fmaf(s[i / D * kTile + j], kv[j * (D + 1) + i % D], x);
-            o[i] = x;
+        const int r0 = lane >> 2;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int32_t i = warp % slices; i < parts; i += slices) {
+            const float4 v = __ldcg(&p.part_o[((spot(i) * MT + ht) * (D / 8) + tile) * 32 + lane]);
+            const float f0 = factor[i][r0], f1 = factor[i][r0 + 8];
+            acc.x += v.x * f0;
+            acc.y += v.y * f0;
+            acc.z += v.z * f1;
+            acc.w += v.w * f1;
+        }
+        sums[warp][lane] = acc;
+        __syncthreads();
+        if (warp % slices == 0) {
+            for (int i = 1; i < slices; ++i) {
+                const float4 v = sums[warp + i][lane];
+                acc.x += v.x;
+                acc.y += v.y;
+                acc.z += v.z;
+                acc.w += v.w;
+            }
+            const int left = p.G - ht * 16;
+            uint32_t *op = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p.out) +
+                                                        ((item * p.G + ht * 16 + r0) * D + tile * 8 + (lane & 3) * 2) * 2);
+            if (r0 < left) op[0] = Num<T>::pack(acc.x, acc.y);
+            if (r0 + 8 < left) op[4 * D] = Num<T>::pack(acc.z, acc.w);
+        }
+        return;
+    }
+    if (parts == 1) {
+        if (tid < p.G) z[tid] = __ldcg(&p.lse2[item * (16 * MT) + tid]);
+    } else {
+        for (int ht = 0; ht < MT; ++ht) {
+            const float lse2 = stats(ht, false);
+            if (lane == 0 && ht * 16 + warp < p.G) z[ht * 16 + warp] = lse2;
         }
     }
     __syncthreads();
-    T *out = (T *)p.out + (b * p.Hk + g) * G * D;
-    for (int i = tid; i < G * D; i += kThreads) out[i] = from_f<T>(l[i / D] != 0.f ? o[i] / l[i / D] : 0.f);
-    for (int i = tid; i < G; i += kThreads) {
-        m[i] = l[i] != 0.f ? m[i] + log2f(l[i]) : -INFINITY;
-        if (p.lse) p.lse[(b * p.Hk + g) * G + i] = m[i] * kLn2;
-    }
-    if (!p.weights) return;
-    for (int64_t p0 = 0; p0 < len; p0 += kTile) {
-        scores(p0);
-        if (tid < kTile && tok[tid] >= 0) {
-            float x = 0.f;
-            for (int h = 0; h < G; ++h)
-                if (m[h] != -INFINITY) x += exp2f(s[h * kTile + tid] - m[h]);
-            p.weights[b * p.w_sb + g * p.w_sh + p0 + tid] += x;
+    const float *sc = p.scores + item * p.G * p.score_ld;
+    float *w = p.weights + b * p.w_sb + g * p.w_sh;
+    const int32_t n_blocks = gridDim.y - splits, mine = blockIdx.y - splits;
+    for (int64_t pos = (int64_t)mine * kJoinThreads + tid; pos < len; pos += (int64_t)n_blocks * kJoinThreads) {
+        float x = 0.f;
+#pragma unroll 8
+        for (int h = 0; h < p.G; ++h) {
+            const float s = __ldcs(sc + h * p.score_ld + pos);
+            x += s == -INFINITY || z[h] == -INFINITY ? 0.f : ex2(s - z[h]);  // positions not held have s = -inf
         }
+        w[pos] += x;
     }
 }
 
-template <typename T, int D> int launch(const Params &p, int64_t B, cudaStream_t s) {
-    const int smem = (2 * p.G * D + kTile * (D + 1) + p.G * kTile + 3 * p.G) * 4;
-    UNUM_CHECK_CUDA(cudaFuncSetAttribute(attend_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
-    attend_kernel<T, D><<<dim3(p.Hk, (unsigned)B), kThreads, smem, s>>>(p);
-    return unum::check_launch("attend_kernel");
+int64_t workers_of_device() {
+    const int64_t n = (int64_t)unum::sm_count() * kBlocksPerSm;
+    return n < kMaxWorkers ? n : kMaxWorkers;
+}
+
+int head_tiles(int64_t G) { return G <= 16 ? 1 : (G <= 32 ? 2 : 4); }
+
+// The workspace's parts, in order; each a multiple of 16 bytes.
+struct Layout {
+    size_t span, lse2, part_ml, part_o, scores, bytes;
+    int64_t score_ld;
+};
+
+Layout layout_of(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t max_len, bool gather) {
+    const int64_t W = workers_of_device(), rows = 16 * head_tiles(Hq / Hk), items = B * Hk;
+    Layout l;
+    size_t at = 0;
+    auto take = [&](int64_t bytes) {
+        const size_t o = at;
+        at += ((size_t)bytes + 15) / 16 * 16;
+        return o;
+    };
+    l.part_o = take(2 * W * rows * D * 4);
+    l.part_ml = take(2 * W * rows * 8);
+    l.span = take(items * 8);
+    l.lse2 = take(items * rows * 4);
+    l.score_ld = (max_len + kUnit - 1) / kUnit * kUnit;
+    l.scores = take(gather ? items * (Hq / Hk) * l.score_ld * 4 : 0);
+    l.bytes = at;
+    return l;
+}
+
+template <typename T, int D, int MT> int launch(const Params &p, cudaStream_t s) {
+    constexpr int kTeams = kWarps / MT;
+    constexpr uint32_t kSlot = 2 * kStep * D * 2;
+    constexpr uint32_t kSlots = kRingBytes / (kTeams * kSlot) > 8 ? 8 : kRingBytes / (kTeams * kSlot);
+    constexpr uint32_t smem = kTeams * kSlots * kSlot + (kTeams > 1 ? 2 * (D / 8) * 32 * 16 : 0);
+    UNUM_CHECK_CUDA(cudaFuncSetAttribute(attend_kernel<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    attend_kernel<T, D, MT><<<(unsigned)p.workers, kThreads, smem, s>>>(p);
+    if (int rc = unum::check_launch("attend_kernel")) return rc;
+    const int64_t items = (int64_t)p.B * p.Hk;
+    // Parts an item has at most: that many blocks share the whole work.  `slices` warps share a column's parts.
+    int slices = 1;
+    while (slices < 16 && slices * 4 * items < p.workers) slices *= 2;
+    int tiles = D / 8;  // of a block: all its warps on one slice, at most
+    if (16 / slices < tiles) tiles = 16 / slices;
+    slices = 16 / tiles;
+    const int splits = MT * (D / 8) / tiles;
+    int64_t gather = 0;
+    if (p.weights) {
+        gather = (4 * (int64_t)p.workers + items - 1) / items;
+        const int64_t most = ((int64_t)p.max_len + kJoinThreads - 1) / kJoinThreads;
+        if (gather > most) gather = most;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)items, (unsigned)(splits + gather));
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    UNUM_CHECK_CUDA(cudaLaunchKernelEx(&cfg, join_kernel<T, D, MT>, p, (int32_t)slices, (int32_t)splits));
+    return unum::check_launch("join_kernel");
+}
+
+template <typename T> int launch_for(const Params &p, int64_t D, cudaStream_t s) {
+    const int mt = head_tiles(p.G);
+    if (D == 128) return mt == 1 ? launch<T, 128, 1>(p, s) : mt == 2 ? launch<T, 128, 2>(p, s) : launch<T, 128, 4>(p, s);
+    return mt == 1 ? launch<T, 64, 1>(p, s) : mt == 2 ? launch<T, 64, 2>(p, s) : launch<T, 64, 4>(p, s);
 }
 
 }  // namespace
 
 extern "C" size_t unum_paged_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t max_seqlen,
                                                       int gather_weights) {
-    (void)B, (void)Hq, (void)Hk, (void)D, (void)max_seqlen, (void)gather_weights;
-    return 16;
+    if (B < 0 || Hq <= 0 || Hk <= 0 || Hq < Hk || D <= 0 || max_seqlen < 0) return 0;
+    return layout_of(B, Hq, Hk, D, max_seqlen, gather_weights != 0).bytes;
 }
 
 extern "C" int unum_paged_attention(const void *q, int64_t B, int64_t Hq, int64_t D, int64_t q_sb, int64_t q_sh,
@@ -171,33 +680,44 @@ extern "C" int unum_paged_attention(const void *q, int64_t B, int64_t Hq, int64_
                    "q, k_cache, v_cache and out must be 16-byte aligned");
     UNUM_CHECK_ARG((q_sb | q_sh | k_st | k_sh | v_st | v_sh) % 8 == 0,
                    "strides of q, k_cache and v_cache must be multiples of 8 elements");
-    UNUM_CHECK_ARG(B < 65536 && Hk < 65536 && B * Hk < ((int64_t)1 << 31), "too many sequences or kv heads");
-    UNUM_CHECK_ARG(max_seqlen < ((int64_t)1 << 31), "max_seqlen must stay below 2^31");
-    if (workspace_bytes < unum_paged_attention_workspace_size(B, Hq, Hk, D, max_seqlen, weights != nullptr) ||
-        !workspace) {
-        unum::set_error("workspace missing or too small (%lld bytes)", (long long)workspace_bytes);
+    UNUM_CHECK_ARG(B < ((int64_t)1 << 31) / Hk && Hk < 65536, "too many sequences or kv heads");
+    UNUM_CHECK_ARG(max_seqlen <= ((int64_t)1 << 31) - 2 * kUnit && n_tokens < ((int64_t)1 << 31),
+                   "max_seqlen and n_tokens must stay below 2^31");
+    const Layout l = layout_of(B, Hq, Hk, D, max_seqlen, weights != nullptr);
+    if (workspace_bytes < l.bytes || !workspace || !unum::aligned16(workspace)) {
+        unum::set_error("workspace missing, misaligned or too small (%lld bytes; %lld needed)", (long long)workspace_bytes,
+                        (long long)l.bytes);
         return UNUM_ERR_WORKSPACE;
     }
     Params p;
-    p.q = q, p.kc = k_cache, p.vc = v_cache;
-    p.q_sb = q_sb, p.q_sh = q_sh, p.k_st = k_st, p.k_sh = k_sh, p.v_st = v_st, p.v_sh = v_sh;
+    p.q = (const uint8_t *)q, p.kc = (const uint8_t *)k_cache, p.vc = (const uint8_t *)v_cache;
+    p.q_sb = 2 * q_sb, p.q_sh = 2 * q_sh, p.k_st = 2 * k_st, p.k_sh = 2 * k_sh, p.v_st = 2 * v_st, p.v_sh = 2 * v_sh;
     p.table = block_table;
     p.lens = seqlens;
     p.bt_stride = bt_stride;
     p.n_tokens = n_tokens;
-    p.max_len = max_seqlen;
+    p.max_len = (int32_t)max_seqlen;
     p.shift = 0;
     while (((int64_t)1 << p.shift) < page_size) ++p.shift;
+    p.B = (int32_t)B;
     p.Hk = (int32_t)Hk;
     p.G = (int32_t)(Hq / Hk);
+    // no more blocks than the lengths can give units to
+    const int64_t most = B * Hk * ((max_seqlen + kUnit - 1) / kUnit), W = workers_of_device();
+    p.workers = (int32_t)(most < 1 ? 1 : (most < W ? most : W));
     p.c = softmax_scale * kLog2e;
     p.out = out;
     p.lse = lse;
     p.weights = weights;
     p.w_sb = w_sb;
     p.w_sh = w_sh;
+    uint8_t *ws = (uint8_t *)workspace;
+    p.span = (int2 *)(ws + l.span);
+    p.lse2 = (float *)(ws + l.lse2);
+    p.part_ml = (float2 *)(ws + l.part_ml);
+    p.part_o = (float4 *)(ws + l.part_o);
+    p.scores = (float *)(ws + l.scores);
+    p.score_ld = l.score_ld;
     cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == UNUM_DTYPE_BF16)
-        return D == 128 ? launch<__nv_bfloat16, 128>(p, B, s) : launch<__nv_bfloat16, 64>(p, B, s);
-    return D == 128 ? launch<__half, 128>(p, B, s) : launch<__half, 64>(p, B, s);
+    return dtype == UNUM_DTYPE_BF16 ? launch_for<__nv_bfloat16>(p, D, s) : launch_for<__half>(p, D, s);
 }
