@@ -196,7 +196,7 @@ def test_evict_entry_refuses(lib, over, rc):
     assert lib.unum_cache_evict(*a.values()) == rc
 
 
-def test_cpu_tensors_are_refused():
+def test_cpu_tensors_are_refused(lib):
     from unum_ops_b200 import append_cache, evict_cache, paged_attention
 
     q, kc, vc, table, lens = make_case(1, [5, 9], 2, 4, 64, 1, "bf16")
@@ -208,15 +208,7 @@ def test_cpu_tensors_are_refused():
         evict_cache(table, lens, torch.zeros(2, 2, table.shape[1]), budget=4)
 
 
-@pytest.fixture
-def no_cuda_needed(monkeypatch):
-    """Lets the wrappers' own checks, which come before any launch, run on CPU tensors."""
-    from unum_ops_b200 import _lib
-
-    monkeypatch.setattr(_lib, "require_cuda", lambda *t: torch.device("cpu"))
-
-
-def test_attention_wrapper_refuses(no_cuda_needed):
+def test_attention_wrapper_refuses(lib):
     from unum_ops_b200 import paged_attention
 
     q, kc, vc, table, lens = make_case(1, [5, 9], 2, 4, 64, 1, "bf16")
@@ -241,7 +233,7 @@ def test_attention_wrapper_refuses(no_cuda_needed):
             paged_attention(a.pop("q"), a.pop("kc"), a.pop("vc"), a.pop("table"), a.pop("lens"), **a)
 
 
-def test_append_and_evict_wrappers_refuse(no_cuda_needed):
+def test_append_and_evict_wrappers_refuse(lib):
     from unum_ops_b200 import append_cache, evict_cache
 
     _, kc, vc, table, lens = make_case(1, [5, 9], 2, 4, 64, 1, "bf16")
@@ -263,14 +255,6 @@ def test_append_and_evict_wrappers_refuse(no_cuda_needed):
         evict_cache(table, lens, w.double(), budget=3)
     with pytest.raises(ValueError):
         evict_cache(table, lens[:1], w, budget=3)
-
-
-def test_views_that_share_no_memory_pass():
-    from unum_ops_b200.paged_cache import _overlaps
-
-    kv = torch.zeros(6, 2, 3, 64)
-    assert not _overlaps(kv[:, 0]) and not _overlaps(kv[:, 1]) and not _overlaps(kv[1:4, 0].transpose(0, 1))
-    assert _overlaps(kv[:1, 0].expand(4, 3, 64)) and _overlaps(torch.zeros(100).as_strided((4, 3, 8), (4, 16, 1)))
 
 
 # ------------------------------------------------------------------------------------------------ attention (GPU)

@@ -1,10 +1,12 @@
-"""Build the CUDA extension in-tree: unum_ops_b200/lib/libunum_ops_b200.so.
+"""Build the CUDA extension in-tree: unum_ops_b200/lib/libunum_ops_b200.so, and its
+binding to torch's tensors, unum_ops_b200/lib/_binding.so.
 
 nvcc compiles every ``csrc/*.cu`` for sm_100a only (``-gencode
 arch=compute_100a,code=sm_100a``) and links one shared library exposing the C
 ABI declared in ``include/unum_ops_b200.h``.  The CUDA runtime is linked as a
 shared library so the extension shares the runtime state (current device,
-streams) of the PyTorch process that loads it.
+streams) of the PyTorch process that loads it.  ``csrc/binding.cpp`` (the native
+half of ``paged_cache``) is host code against torch's headers, linked to that library.
 
 Usage: ``python -m unum_ops_b200._build [--force]``.
 """
@@ -20,6 +22,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(OUT_DIR, "libunum_ops_b200.so")
+BINDING = os.path.join(OUT_DIR, "_binding.so")
 ROOT = os.path.dirname(HERE)
 
 NVCC_FLAGS = [
@@ -40,15 +43,31 @@ def _sources():
 
 
 def _deps():
-    return [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh"))] + [
+    return [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh", ".cpp"))] + [
         os.path.join(ROOT, "include", "unum_ops_b200.h")]
 
 
 def needs_build() -> bool:
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(BINDING):
         return True
-    t = os.path.getmtime(LIB)
+    t = min(os.path.getmtime(LIB), os.path.getmtime(BINDING))
     return any(os.path.getmtime(d) > t for d in _deps())
+
+
+def _binding_command(src, out):
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cxx = os.environ.get("CXX") or shutil.which("g++") or "c++"
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    inc = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    libs = cpp_extension.library_paths()
+    return [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-isystem{i}" for i in inc], src, "-o", out,
+            *[f"-L{d}" for d in libs], "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+            "-L" + OUT_DIR, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -80,6 +99,11 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stderr}")
     os.replace(tmp, LIB)
+    tmp = BINDING + ".tmp"
+    r = subprocess.run(_binding_command(os.path.join(CSRC, "binding.cpp"), tmp), capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"binding failed:\n{r.stderr}")
+    os.replace(tmp, BINDING)
     return LIB
 
 

@@ -6,6 +6,7 @@ tensor is not on a CUDA device, the wrappers raise.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 
 import torch
@@ -96,6 +97,25 @@ def load() -> ctypes.CDLL:
             fn.restype = res
         _lib = L
     return _lib
+
+
+_native = None
+
+
+def binding():
+    """The native half of paged_cache, on top of the CUDA library (raises if it has not been built)."""
+    global _native
+    if _native is None:
+        load()
+        path = _build.BINDING
+        if not os.path.exists(path):
+            raise RuntimeError(f"unum_ops_b200 binding not found at {path}; build it with "
+                               "`python -m unum_ops_b200._build` (there is no CPU fallback)")
+        spec = importlib.util.spec_from_file_location("_binding", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _native = module
+    return _native
 
 
 def check(rc: int) -> None:

@@ -1,0 +1,319 @@
+// Native half of unum_ops_b200/paged_cache.py: checks of arguments, allocation and the C ABI's calls.
+//
+// A decode step calls these operators for every layer, and its kernels run for a few microseconds; the same checks and
+// allocations in Python, with the C ABI called through ctypes, took 24 us (append_cache) and 32 us (paged_attention) a
+// call on the host, several times the kernels' own time.  Here a call takes its tensors as they are: no Python object is
+// made on the way but the results.
+#define PY_SSIZE_T_CLEAN
+#include <Python.h>
+
+#include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
+#include <c10/cuda/CUDACachingAllocator.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+#include <vector>
+
+#include "../../include/unum_ops_b200.h"
+
+namespace {
+
+using at::Tensor;
+
+// A refusal on its way to Python: the exception's type and message.
+struct Refused {
+    PyObject *type;
+    std::string what;
+};
+
+std::string text(const char *s) { return s; }
+std::string text(int64_t x) { return std::to_string(x); }
+std::string text(at::ScalarType x) { return c10::toString(x); }
+std::string text(c10::Device x) { return x.str(); }
+std::string text(at::IntArrayRef x) {
+    std::string s = "[";
+    for (size_t i = 0; i < x.size(); ++i) s += (i ? ", " : "") + std::to_string(x[i]);
+    return s + "]";
+}
+
+template <typename... A> [[noreturn]] void refuse(PyObject *type, const A &...a) {
+    std::string s;
+    (void)std::initializer_list<int>{(s += text(a), 0)...};
+    throw Refused{type, s};
+}
+
+// Arguments in order, each taken by its name.
+struct Args {
+    PyObject *const *a;
+    Tensor none;
+    const Tensor &tensor(int i, const char *name) const {
+        if (!THPVariable_Check(a[i])) refuse(PyExc_TypeError, name, " must be a tensor");
+        return THPVariable_Unpack(a[i]);
+    }
+    const Tensor &optional_tensor(int i, const char *name) const { return a[i] == Py_None ? none : tensor(i, name); }
+    int64_t integer(int i, const char *name) const {
+        PyObject *v = PyNumber_Index(a[i]);
+        const int64_t x = v ? PyLong_AsLongLong(v) : -1;
+        Py_XDECREF(v);
+        if (PyErr_Occurred()) {
+            PyErr_Clear();
+            refuse(PyExc_TypeError, name, " must be an integer");
+        }
+        return x;
+    }
+    double number(int i, const char *name) const {
+        const double x = PyFloat_AsDouble(a[i]);
+        if (PyErr_Occurred()) {
+            PyErr_Clear();
+            refuse(PyExc_TypeError, name, " must be a number");
+        }
+        return x;
+    }
+    bool truth(int i) const { return PyObject_IsTrue(a[i]) == 1; }
+};
+
+void no_grad(std::initializer_list<const Tensor *> ts) {
+    if (!at::GradMode::is_enabled()) return;
+    for (const Tensor *t : ts)
+        if (t->defined() && t->requires_grad())
+            refuse(PyExc_NotImplementedError,
+                   "the paged cache's operators have no backward pass: call them under torch.no_grad()");
+}
+
+// Called after the other checks, so that those are the same on a machine without a GPU.
+c10::Device on_one_gpu(std::initializer_list<const Tensor *> ts) {
+    const Tensor &first = **ts.begin();
+    for (const Tensor *t : ts) {
+        if (!t->defined()) continue;
+        if (!t->is_cuda())
+            refuse(PyExc_ValueError, "unum_ops_b200 runs on CUDA tensors only; got a tensor on ", t->device());
+        if (t->device() != first.device())
+            refuse(PyExc_ValueError, "tensors on different devices: ", first.device(), " and ", t->device());
+    }
+    return first.device();
+}
+
+void check(int rc) {
+    if (rc == UNUM_OK) return;
+    if (rc == UNUM_ERR_INVALID) refuse(PyExc_ValueError, unum_last_error());
+    if (rc == UNUM_ERR_UNSUPPORTED) refuse(PyExc_NotImplementedError, unum_last_error());
+    refuse(PyExc_RuntimeError, "unum_ops_b200 error ", (int64_t)rc, ": ", unum_last_error());
+}
+
+// The stride of dim d in elements; 0 for a dim of one element (whose stride says nothing).
+int64_t stride(const Tensor &t, int d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+
+// Whether 16-byte loads can read the rows of a 3-d tensor of 2-byte elements.
+bool has_rows16(const Tensor &t) {
+    return t.stride(2) == 1 && (stride(t, 0) | stride(t, 1)) % 8 == 0 &&
+           reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+}
+
+Tensor rows16(const Tensor &t) { return has_rows16(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+
+// Whether two elements may share memory (an expanded or an overlapping view).
+bool overlaps(const Tensor &t) {
+    if (t.is_contiguous()) return false;
+    std::vector<std::pair<int64_t, int64_t>> dims;  // stride, size
+    for (int64_t d = 0; d < t.dim(); ++d)
+        if (t.size(d) > 1) dims.emplace_back(t.stride(d), t.size(d));
+    std::sort(dims.begin(), dims.end());
+    int64_t reach = 0;
+    for (const auto &d : dims) {
+        if (d.first <= reach) return true;
+        reach += (d.second - 1) * d.first;
+    }
+    return false;
+}
+
+Tensor as_i32(const Tensor &t) { return (t.scalar_type() == at::kInt ? t : t.to(at::kInt)).contiguous(); }
+
+void check_cache(const Tensor &k, const Tensor &v) {
+    const char *name = "k_cache";
+    for (const Tensor *c : {&k, &v}) {
+        if (c->dim() != 3) refuse(PyExc_ValueError, name, " must be [n_tokens, Hk, D]; got ", c->sizes());
+        if (c->scalar_type() != at::kBFloat16 && c->scalar_type() != at::kHalf)
+            refuse(PyExc_ValueError, name, " must be bfloat16 or float16; got ", c->scalar_type());
+        if (!has_rows16(*c))
+            refuse(PyExc_ValueError, name, " must have contiguous, 16-byte aligned rows; got strides ", c->strides());
+        name = "v_cache";
+    }
+    if (k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type())
+        refuse(PyExc_ValueError, "k_cache and v_cache differ: ", k.sizes(), " ", k.scalar_type(), " and ", v.sizes(), " ",
+               v.scalar_type());
+}
+
+void check_table(const Tensor &t, int64_t page_size) {
+    if (t.dim() != 2) refuse(PyExc_ValueError, "block_table must be [B, n_pages]; got ", t.sizes());
+    if (page_size < 1 || (page_size & (page_size - 1)) || page_size > 65536)
+        refuse(PyExc_ValueError, "page_size must be a power of two up to 65536; got ", page_size);
+}
+
+Tensor table_i32(const Tensor &t) {
+    const Tensor x = t.scalar_type() == at::kInt ? t : t.to(at::kInt);
+    return x.stride(1) == 1 || x.size(1) < 2 ? x : x.contiguous();
+}
+
+void written(const Tensor &t) {  // for whoever has saved it
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+void *stream_of(c10::Device d) { return c10::cuda::getCurrentCUDAStream(d.index()).stream(); }
+
+// append_cache(k, v, k_cache, v_cache, block_table, token_to_bs, token_pos_in_bs, page_size)
+PyObject *append_cache(const Args &a) {
+    const Tensor &k = a.tensor(0, "k"), &v = a.tensor(1, "v"), &kc = a.tensor(2, "k_cache"), &vc = a.tensor(3, "v_cache");
+    const Tensor &table = a.tensor(4, "block_table"), &bs = a.tensor(5, "token_to_bs"), &pos = a.tensor(6, "token_pos_in_bs");
+    const int64_t page = a.integer(7, "page_size");
+    no_grad({&k, &v, &kc, &vc});
+    check_cache(kc, vc);
+    if (k.dim() != 3 || k.sizes() != v.sizes() || k.size(1) != kc.size(1) || k.size(2) != kc.size(2))
+        refuse(PyExc_ValueError, "k and v must be [T, ", kc.size(1), ", ", kc.size(2), "] like the cache's rows; got ",
+               k.sizes(), " and ", v.sizes());
+    if (k.scalar_type() != kc.scalar_type() || v.scalar_type() != kc.scalar_type())
+        refuse(PyExc_ValueError, "k and v must have the cache's dtype ", kc.scalar_type(), "; got ", k.scalar_type(), " and ",
+               v.scalar_type());
+    if (overlaps(kc) || overlaps(vc) || (kc.numel() && kc.const_data_ptr() == vc.const_data_ptr()))
+        refuse(PyExc_ValueError, "k_cache and v_cache are written to: their rows must not share memory");
+    const int64_t T = k.size(0);
+    if (bs.numel() != T || pos.numel() != T)
+        refuse(PyExc_ValueError, "token_to_bs and token_pos_in_bs must have one entry for each of ", T, " tokens; got ",
+               bs.numel(), " and ", pos.numel());
+    check_table(table, page);
+    const c10::Device dev = on_one_gpu({&k, &v, &kc, &vc, &table, &bs, &pos});
+    if (k.numel() == 0) Py_RETURN_NONE;
+    const c10::cuda::CUDAGuard guard(dev);
+    const Tensor k_ = rows16(k), v_ = rows16(v), t = table_i32(table), bs_ = as_i32(bs), pos_ = as_i32(pos);
+    check(unum_cache_append(k_.const_data_ptr(), v_.const_data_ptr(), T, k_.size(1), k_.size(2), stride(k_, 0), stride(k_, 1),
+                            stride(v_, 0), stride(v_, 1), kc.data_ptr(), vc.data_ptr(), kc.size(0), stride(kc, 0),
+                            stride(kc, 1), stride(vc, 0), stride(vc, 1), t.const_data_ptr<int32_t>(), t.size(0), t.size(1),
+                            t.stride(0), page, bs_.const_data_ptr<int32_t>(), pos_.const_data_ptr<int32_t>(),
+                            stream_of(dev)));
+    written(kc);
+    written(vc);
+    Py_RETURN_NONE;
+}
+
+// paged_attention(q, k_cache, v_cache, block_table, seqlens, page_size, max_seqlen, softmax_scale, weights, return_lse)
+PyObject *paged_attention(const Args &a) {
+    const Tensor &q = a.tensor(0, "q"), &kc = a.tensor(1, "k_cache"), &vc = a.tensor(2, "v_cache");
+    const Tensor &table = a.tensor(3, "block_table"), &lens = a.tensor(4, "seqlens");
+    const int64_t page = a.integer(5, "page_size");
+    const Tensor &weights = a.optional_tensor(8, "weights");
+    no_grad({&q, &kc, &vc, &weights});
+    check_cache(kc, vc);
+    if (q.dim() != 3 || q.size(2) != kc.size(2))
+        refuse(PyExc_ValueError, "q must be [B, Hq, ", kc.size(2), "]; got ", q.sizes());
+    const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2), Hk = kc.size(1);
+    if (q.scalar_type() != kc.scalar_type())
+        refuse(PyExc_ValueError, "q must have the cache's dtype ", kc.scalar_type(), "; got ", q.scalar_type());
+    if (Hk == 0 || Hq == 0 || Hq % Hk)
+        refuse(PyExc_ValueError, Hq, " query heads are no multiple of ", Hk, " kv heads");
+    check_table(table, page);
+    if (table.size(0) != B || lens.numel() != B)
+        refuse(PyExc_ValueError, "block_table and seqlens must have one row for each of ", B, " sequences; got ",
+               table.size(0), " and ", lens.numel());
+    int64_t max_len = table.size(1) * page;
+    if (a.a[6] != Py_None) max_len = std::min(max_len, a.integer(6, "max_seqlen"));
+    if (max_len < 0) refuse(PyExc_ValueError, "max_seqlen must not be negative; got ", max_len);
+    if (weights.defined()) {
+        if (weights.dim() != 3 || weights.size(0) != B || weights.size(1) != Hk || weights.size(2) < max_len)
+            refuse(PyExc_ValueError, "weights must be [", B, ", ", Hk, ", >= ", max_len, "]; got ", weights.sizes());
+        if (weights.scalar_type() != at::kFloat || (weights.stride(2) != 1 && weights.size(2) > 1) || overlaps(weights))
+            refuse(PyExc_ValueError, "weights must be float32 with contiguous rows that share no memory");
+    }
+    const double scale = a.a[7] == Py_None ? 1.0 / std::sqrt((double)D) : a.number(7, "softmax_scale");
+    const c10::Device dev = on_one_gpu({&q, &kc, &vc, &table, &lens, &weights});
+    const c10::cuda::CUDAGuard guard(dev);
+    const Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+    Tensor lse;
+    if (a.truth(9)) lse = at::empty({B, Hq}, q.options().dtype(at::kFloat));
+    if (B) {
+        const Tensor q_ = rows16(q), t = table_i32(table), lens_ = as_i32(lens);
+        const size_t bytes = unum_paged_attention_workspace_size(B, Hq, Hk, D, max_len, weights.defined());
+        // a call's own: calls on other streams, or of other graphs, may run at the same time
+        const c10::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
+        check(unum_paged_attention(
+            q_.const_data_ptr(), B, Hq, D, stride(q_, 0), stride(q_, 1), kc.const_data_ptr(), vc.const_data_ptr(),
+            q.scalar_type() == at::kHalf ? UNUM_DTYPE_F16 : UNUM_DTYPE_BF16, kc.size(0), Hk, stride(kc, 0), stride(kc, 1),
+            stride(vc, 0), stride(vc, 1), t.const_data_ptr<int32_t>(), t.size(1), t.stride(0), page,
+            lens_.const_data_ptr<int32_t>(), max_len, (float)scale, out.data_ptr(), lse.defined() ? lse.data_ptr<float>() : nullptr,
+            weights.defined() ? weights.data_ptr<float>() : nullptr, weights.defined() ? weights.stride(0) : 0,
+            weights.defined() ? weights.stride(1) : 0, ws.get(), bytes, stream_of(dev)));
+        if (weights.defined()) written(weights);
+    }
+    if (!lse.defined()) return THPVariable_Wrap(out);
+    return Py_BuildValue("(NN)", THPVariable_Wrap(out), THPVariable_Wrap(lse));
+}
+
+// evict_cache(block_table, seqlens, weights, budget, init_pages, local_pages, page_size)
+PyObject *evict_cache(const Args &a) {
+    const Tensor &table = a.tensor(0, "block_table"), &lens = a.tensor(1, "seqlens"), &weights = a.tensor(2, "weights");
+    const int64_t budget = a.integer(3, "budget"), init = a.integer(4, "init_pages"), local = a.integer(5, "local_pages");
+    const int64_t page = a.integer(6, "page_size");
+    no_grad({&weights});
+    check_table(table, page);
+    const int64_t B = table.size(0), n_pages = table.size(1);
+    if (lens.numel() != B)
+        refuse(PyExc_ValueError, "seqlens must have one entry for each of ", B, " sequences; got ", lens.numel());
+    if (weights.dim() != 3 || weights.size(0) != B || weights.size(1) < 1 || weights.size(2) != n_pages * page)
+        refuse(PyExc_ValueError, "weights must be [", B, ", Hk, ", n_pages * page, "]; got ", weights.sizes());
+    if (weights.scalar_type() != at::kFloat)
+        refuse(PyExc_ValueError, "weights must be float32; got ", weights.scalar_type());
+    if (local < 1 || init < 0 || budget < 0 || budget - init < local)
+        refuse(PyExc_ValueError, "need init_pages >= 0, local_pages >= 1 and budget >= their sum; got budget ", budget,
+               ", init_pages ", init, ", local_pages ", local);
+    const c10::Device dev = on_one_gpu({&table, &lens, &weights});
+    const c10::cuda::CUDAGuard guard(dev);
+    const auto ints = weights.options().dtype(at::kInt);
+    const Tensor new_table = at::empty({B, n_pages}, ints), new_lens = at::empty({B}, ints);
+    const Tensor new_w = at::empty(weights.sizes(), weights.options().memory_format(at::MemoryFormat::Contiguous));
+    const Tensor gone = at::empty({B, n_pages}, ints);
+    if (B) {
+        const Tensor t = table_i32(table), lens_ = as_i32(lens);
+        const Tensor w = weights.stride(2) == 1 || weights.size(2) < 2 ? weights : weights.contiguous();
+        check(unum_cache_evict(t.const_data_ptr<int32_t>(), B, n_pages, t.stride(0), lens_.const_data_ptr<int32_t>(),
+                               w.const_data_ptr<float>(), w.size(1), w.stride(0), w.stride(1), page, budget, init, local,
+                               new_table.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(), new_w.data_ptr<float>(),
+                               gone.data_ptr<int32_t>(), stream_of(dev)));
+    }
+    return Py_BuildValue("(NNNN)", THPVariable_Wrap(new_table), THPVariable_Wrap(new_lens), THPVariable_Wrap(new_w),
+                         THPVariable_Wrap(gone));
+}
+
+template <PyObject *(*kFn)(const Args &), int kArgs>
+PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    try {
+        if (n != kArgs) refuse(PyExc_TypeError, "expected ", (int64_t)kArgs, " arguments, got ", (int64_t)n);
+        return kFn(Args{args, {}});
+    } catch (const Refused &r) {
+        PyErr_SetString(r.type, r.what.c_str());
+    } catch (const c10::OutOfMemoryError &e) {
+        PyObject *torch = PyImport_ImportModule("torch");
+        PyObject *type = torch ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;
+        if (type) PyErr_SetString(type, e.what_without_backtrace());
+        Py_XDECREF(type);
+        Py_XDECREF(torch);
+    } catch (const c10::Error &e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
+    } catch (const std::exception &e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (...) {
+        PyErr_SetString(PyExc_RuntimeError, "unknown C++ exception");
+    }
+    return nullptr;
+}
+
+#define ENTRY(name, n) {#name, reinterpret_cast<PyCFunction>(entry<name, n>), METH_FASTCALL, nullptr}
+PyMethodDef kMethods[] = {ENTRY(append_cache, 8), ENTRY(paged_attention, 10), ENTRY(evict_cache, 7),
+                          {nullptr, nullptr, 0, nullptr}};
+PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__binding(void) { return PyModule_Create(&kModule); }
