@@ -37,7 +37,6 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kBlocksPerSm = 2;
 constexpr int kUnit = 64;            // positions dealt to a block at a time
-constexpr int kStep = 16;            // positions of a team's step: a unit is kWarps steps of 16
 constexpr int kGrain = 2;            // units a block takes at least: below it the join costs more than the split gains
 constexpr int kMaxWorkers = 512;     // resident blocks, at most
 constexpr uint32_t kRingBytes = 96 * 1024;
@@ -48,9 +47,10 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 struct Params {
     const uint8_t *q, *kc, *vc;
-    int64_t q_sb, q_sh, k_st, k_sh, v_st, v_sh;  // bytes
+    int64_t q_sb, q_sh, k_sh, v_sh;  // bytes
     const int32_t *table, *lens;
     int64_t bt_stride, n_tokens;
+    int32_t k_st, v_st;              // bytes
     int32_t max_len, shift, B, Hk, G, workers;
     float c;  // scale * log2(e)
     void *out;
@@ -68,7 +68,11 @@ struct Params {
 // ---------------------------------------------------------------------------------------------- instructions
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes) {
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// 16 zero bytes where `bytes` is 0
+__device__ __forceinline__ void cp_async16_if(uint32_t dst, const void *src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -144,19 +148,19 @@ struct Place {
 
 // Units before this thread's share of the sequences, and the total (over one kv head).  All threads call it.
 template <int kN>
-__device__ __forceinline__ int64_t scan_units(const Params &p, int32_t b0, int32_t b1, int64_t *warp_sums, int64_t &total) {
+__device__ __forceinline__ int32_t scan_units(const Params &p, int32_t b0, int32_t b1, int32_t *warp_sums, int32_t &total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t mine = 0;
+    int32_t mine = 0;
     for (int32_t b = b0; b < b1; ++b) mine += units_of(length(p, b));
-    int64_t x = mine;
+    int32_t x = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        const int32_t y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
     if (lane == 31) warp_sums[warp] = x;
     __syncthreads();
-    int64_t before = x - mine;
+    int32_t before = x - mine;
     total = 0;
 #pragma unroll
     for (int w = 0; w < kN; ++w) {
@@ -166,26 +170,45 @@ __device__ __forceinline__ int64_t scan_units(const Params &p, int32_t b0, int32
     return before;
 }
 
+// The units are dealt out in a row: the first `more` blocks have base + 1 of them, the others base.
+struct Shares {
+    int32_t base, more;
+    __device__ __forceinline__ Shares(int32_t total, int32_t workers) : base(total / workers), more(total % workers) {}
+    __device__ __forceinline__ int32_t begin(int32_t w) const { return w * base + min(w, more); }
+    __device__ __forceinline__ int32_t owner(int32_t u) const {
+        const int32_t edge = more * (base + 1);
+        return u < edge ? u / (base + 1) : more + (u - edge) / base;
+    }
+};
+
 template <int MT> __device__ __forceinline__ void team_sync(int team) {
     if (MT == 1) __syncwarp();
     else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(MT * 32) : "memory");
 }
 
-// MT = 16-head tiles of a group (1, 2 or 4): the warps of a team.
+// MT = 16-head tiles of a group (1, 2 or 4): the warps of a team.  A team's step is 16 positions, or 32 where a team has
+// several warps and so more room in the ring: the steps' barriers, maxima and copies cost half as much a position.
+template <int D, int MT> struct Shape {
+    static constexpr int kTeams = kWarps / MT, kStep = MT == 1 ? 16 : 32, kRow = D * 2;  // kRow in bytes
+    static constexpr int kSteps = kUnit / (kTeams * kStep);                               // a team's steps in a unit
+    static constexpr uint32_t kHalf = kStep * kRow, kSlot = 2 * kHalf;                    // keys, values of a step
+    static constexpr int kFit = kRingBytes / (kTeams * kSlot), kSlots = kFit > 8 ? 8 : kFit;
+    static constexpr uint32_t kMerge = kTeams > 1 ? 2 * (D / 8) * 32 * 16 : 0;
+    static constexpr uint32_t kSmem = kTeams * kSlots * kSlot + kMerge;
+};
+
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __grid_constant__ Params p) {
-    constexpr int kTeams = kWarps / MT;
-    constexpr int kRow = D * 2;                          // bytes
-    constexpr uint32_t kHalf = kStep * kRow, kSlot = 2 * kHalf;  // keys, values of a step
-    constexpr int kSlots = kRingBytes / (kTeams * kSlot) > 8 ? 8 : kRingBytes / (kTeams * kSlot);
+    using S = Shape<D, MT>;
+    constexpr int kTeams = S::kTeams, kStep = S::kStep, kSlots = S::kSlots, kRow = S::kRow;
+    constexpr uint32_t kHalf = S::kHalf, kSlot = S::kSlot;
     constexpr int kLanes = kRow / 16, kRows = 32 / kLanes;  // lanes of a row, rows of one copy instruction
     constexpr int kCopies = kStep / kRows / MT;             // of each warp, for keys and for values
     static_assert(kCopies >= 1 && kSlots >= 3, "a step must give every warp a copy");
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ uint32_t held[kTeams][8];                 // which of a slot's positions are valid
-    __shared__ int64_t warp_sums[kWarps];
-    __shared__ int32_t start[3];
-    __shared__ float2 merge_ml[2][16 * 2];
+    __shared__ int32_t warp_sums[kWarps], start[3];
+    __shared__ float2 merge_ml[2][16];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, team = warp / MT, ht = warp % MT;
     const uint32_t ring = smem_u32(smem) + team * (kSlots * kSlot);
     float4 *merge = reinterpret_cast<float4 *>(smem + kTeams * kSlots * kSlot);  // [2][D / 8][32]
@@ -194,22 +217,20 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
     // this block's share of the units
     const int32_t per = (p.B + kThreads - 1) / kThreads;
     const int32_t b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
-    int64_t total, before = scan_units<kWarps>(p, b0, b1, warp_sums, total);
+    int32_t total, before = scan_units<kWarps>(p, b0, b1, warp_sums, total);
     before *= p.Hk;
     total *= p.Hk;
-    int64_t workers = (total + kGrain - 1) / kGrain;
-    if (workers > p.workers) workers = p.workers;
-    const int64_t me = blockIdx.x;
+    const int32_t workers = min((total + kGrain - 1) / kGrain, p.workers), me = blockIdx.x;
     if (me >= workers) return;
-    const int64_t u0 = me * total / workers, u1 = (me + 1) * total / workers;
+    const Shares shares(total, workers);
+    const int32_t u0 = shares.begin(me), u1 = shares.begin(me + 1);
     for (int32_t b = b0; b < b1; ++b) {
-        const int32_t n = units_of(length(p, b));
-        const int64_t mine = (int64_t)n * p.Hk;
+        const int32_t n = units_of(length(p, b)), mine = n * p.Hk;
         if (u0 >= before && u0 < before + mine) {
-            const int64_t r = u0 - before;
+            const int32_t r = u0 - before;
             start[0] = b;
-            start[1] = (int32_t)(r / n);
-            start[2] = (int32_t)(r % n);
+            start[1] = r / n;
+            start[2] = r % n;
         }
         before += mine;
     }
@@ -219,43 +240,53 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
     in.h = start[1];
     in.unit = start[2];
     Place at = in;  // where the arithmetic is
-    const int64_t steps = (u1 - u0) * MT;
-    int64_t fetched = 0;
+    int32_t to_fetch = (u1 - u0) * S::kSteps;
     int in_k = 0;
 
-    // the next step's token of position lane % 16 (or -1), read ahead of its copies
+    // the next step's token of position lane % kStep (or -1), read ahead of its copies
     int32_t tok = -1, tok_h = 0;
     auto fetch = [&]() {
         tok = -1;
-        if (fetched >= steps) return;
-        const int32_t pos = in.unit * kUnit + (team + kTeams * in_k) * kStep + (lane & 15);
+        if (to_fetch == 0) return;
+        const int32_t pos = in.unit * kUnit + (team + kTeams * in_k) * kStep + (lane & (kStep - 1));
         tok_h = in.h;
         if (pos < in.len) {
             const int64_t page = __ldg(p.table + in.b * p.bt_stride + (pos >> p.shift));
             const int64_t t = (page << p.shift) + (pos & ((1 << p.shift) - 1));
             tok = page >= 0 && t < p.n_tokens ? (int32_t)t : -1;
         }
-        ++fetched;
-        if (++in_k == MT) {
+        --to_fetch;
+        if (++in_k == S::kSteps) {
             in_k = 0;
             in.next(p);
         }
     };
-    // its copies into a slot
+    // its copies into a slot.  Where all positions are held the copies need no checks; rows of others are zeroed, since
+    // what their memory held would reach the output as 0 * NaN.
+    constexpr uint32_t kAll = kStep == 32 ? 0xffffffffu : 0xffffu;
+    const int copy_row = ht * kRows + lane / kLanes;
+    const uint32_t copy_to = ring + copy_row * kRow;
+    const uint32_t copy_chunk = lane % kLanes;
     auto issue = [&](uint32_t slot) {
-        const uint32_t mask = __ballot_sync(0xffffffffu, tok >= 0) & 0xffffu;
+        const uint32_t mask = __ballot_sync(0xffffffffu, tok >= 0) & kAll;
         if (ht == 0 && lane == 0) held[team][slot] = mask;
         if (mask) {
-            const uint8_t *kb = p.kc + (int64_t)tok_h * p.k_sh + (lane % kLanes) * 16;
-            const uint8_t *vb = p.vc + (int64_t)tok_h * p.v_sh + (lane % kLanes) * 16;
+            const uint8_t *kb = p.kc + tok_h * p.k_sh + copy_chunk * 16;
+            const uint8_t *vb = p.vc + tok_h * p.v_sh + copy_chunk * 16;
+            const uint32_t to = copy_to + slot * kSlot;
 #pragma unroll
             for (int i = 0; i < kCopies; ++i) {
-                const int row = (i * MT + ht) * kRows + lane / kLanes;
+                const int row = i * MT * kRows + copy_row;
                 const int32_t t = __shfl_sync(0xffffffffu, tok, row);
-                const uint32_t dst = ring + slot * kSlot + row * kRow + (((lane % kLanes) ^ (row & 7)) << 4);
-                const int64_t o = t < 0 ? 0 : t;
-                cp_async16(dst, kb + o * p.k_st, t < 0 ? 0u : 16u);
-                cp_async16(dst + kHalf, vb + o * p.v_st, t < 0 ? 0u : 16u);
+                const uint32_t dst = to + i * MT * kRows * kRow + ((copy_chunk ^ (row & 7)) << 4);
+                if (mask == kAll) {
+                    cp_async16(dst, kb + (int64_t)t * p.k_st);
+                    cp_async16(dst + kHalf, vb + (int64_t)t * p.v_st);
+                } else {
+                    const int64_t o = t < 0 ? 0 : t;
+                    cp_async16_if(dst, kb + o * p.k_st, t < 0 ? 0u : 16u);
+                    cp_async16_if(dst + kHalf, vb + o * p.v_st, t < 0 ? 0u : 16u);
+                }
             }
         }
         cp_commit();
@@ -268,13 +299,17 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
 
     uint32_t slot = 0;
     const int r0 = lane >> 2, c0 = (lane & 3) * 2;
-    int64_t u = u0;
+    // rows and swizzled 16-byte chunks of the matrices that this lane addresses; chunk 2 kk + e is that xor 2 kk
+    const int k_row = (lane & 7) + ((lane >> 4) << 3), v_row = lane & 15;
+    const uint32_t k_at = k_row * kRow + ((((lane >> 3) & 1) ^ (k_row & 7)) << 4);
+    const uint32_t v_at = v_row * kRow + (((lane >> 4) ^ (v_row & 7)) << 4);
+    int32_t u = u0;
     while (u < u1) {
         // one item's units in this block
-        const int64_t seg_end = min(u + (at.units - at.unit), u1);
+        const int32_t seg_end = min(u + (at.units - at.unit), u1);
         const bool from_start = at.unit == 0, to_end = u + (at.units - at.unit) == seg_end;
         const int64_t item = (int64_t)at.b * p.Hk + at.h;
-        const int64_t item_u0 = u - at.unit;
+        const int32_t item_u0 = u - at.unit;
         uint32_t qa[D / 16][4];
         {
             const uint8_t *qb = p.q + at.b * p.q_sb + (int64_t)(at.h * p.G + ht * 16) * p.q_sh + c0 * 2;
@@ -296,35 +331,45 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
 
         for (; u < seg_end; ++u, ++at.unit) {
 #pragma unroll 1
-            for (int k = 0; k < MT; ++k) {
+            for (int k = 0; k < S::kSteps; ++k) {
                 cp_wait<kSlots - 2>();
                 team_sync<MT>(team);  // the slot is filled, and nobody reads the one before it any more
                 issue(slot == 0 ? kSlots - 1 : slot - 1);
                 const uint32_t mask = held[team][slot];
-                const uint32_t kb = ring + slot * kSlot, vb = kb + kHalf;
+                const uint32_t kb = ring + slot * kSlot + k_at, vb = ring + slot * kSlot + kHalf + v_at;
                 slot = slot + 1 == kSlots ? 0 : slot + 1;
                 if (mask == 0 && !p.weights) continue;
-                float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-                if (mask) {
-                    const int row = (lane & 7) + ((lane >> 4) << 3);
+                float s[kStep / 8][4];
 #pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk) {
-                        uint32_t f[4];
-                        ldsm4(f, kb + row * kRow + (((2 * kk + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
-                        Num<T>::mma(s[0], qa[kk], f[0], f[1]);
-                        Num<T>::mma(s[1], qa[kk], f[2], f[3]);
-                    }
+                for (int t = 0; t < kStep / 8; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+                if (mask) {
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+                        for (int t = 0; t < kStep / 16; ++t) {
+                            uint32_t f[4];
+                            ldsm4(f, (kb ^ (kk << 5)) + t * 16 * kRow);
+                            Num<T>::mma(s[2 * t], qa[kk], f[0], f[1]);
+                            Num<T>::mma(s[2 * t + 1], qa[kk], f[2], f[3]);
+                        }
                 }
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < kStep / 8; ++t)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s[t][e] = (mask >> (8 * t + c0 + (e & 1))) & 1u ? s[t][e] * p.c : -INFINITY;
+                    for (int e = 0; e < 4; ++e) s[t][e] *= p.c;
+                if (mask != kAll) {
+                    const uint32_t mine = mask >> c0;
+#pragma unroll
+                    for (int t = 0; t < kStep / 8; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (!((mine >> (8 * t + (e & 1))) & 1u)) s[t][e] = -INFINITY;
+                }
                 if (p.weights) {
                     const int64_t pos = (int64_t)at.unit * kUnit + (team + kTeams * k) * kStep;
                     if (pos < at.len) {
 #pragma unroll
-                        for (int t = 0; t < 2; ++t) {
+                        for (int t = 0; t < kStep / 8; ++t) {
                             if (ht * 16 + r0 < p.G)
                                 *reinterpret_cast<float2 *>(sc + pos + 8 * t) = make_float2(s[t][0], s[t][1]);
                             if (ht * 16 + r0 + 8 < p.G)
@@ -334,8 +379,12 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
                     }
                     if (mask == 0) continue;
                 }
-                float x0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-                float x1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+                float x0 = fmaxf(s[0][0], s[0][1]), x1 = fmaxf(s[0][2], s[0][3]);
+#pragma unroll
+                for (int t = 1; t < kStep / 8; ++t) {
+                    x0 = fmaxf(x0, fmaxf(s[t][0], s[t][1]));
+                    x1 = fmaxf(x1, fmaxf(s[t][2], s[t][3]));
+                }
 #pragma unroll
                 for (int i = 1; i <= 2; i <<= 1) {
                     x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, i));
@@ -359,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
                 }
                 const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
+                for (int t = 0; t < kStep / 8; ++t) {
                     s[t][0] = ex2(s[t][0] - z0);
                     s[t][1] = ex2(s[t][1] - z0);
                     s[t][2] = ex2(s[t][2] - z1);
@@ -367,15 +416,18 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
                     l0 += s[t][0] + s[t][1];
                     l1 += s[t][2] + s[t][3];
                 }
-                uint32_t a[4] = {Num<T>::pack(s[0][0], s[0][1]), Num<T>::pack(s[0][2], s[0][3]),
-                                 Num<T>::pack(s[1][0], s[1][1]), Num<T>::pack(s[1][2], s[1][3])};
-                const int row = lane & 15;
 #pragma unroll
-                for (int nn = 0; nn < D / 16; ++nn) {
-                    uint32_t f[4];
-                    ldsm4t(f, vb + row * kRow + (((2 * nn + (lane >> 4)) ^ (row & 7)) << 4));
-                    Num<T>::mma(o[2 * nn], a, f[0], f[1]);
-                    Num<T>::mma(o[2 * nn + 1], a, f[2], f[3]);
+                for (int t = 0; t < kStep / 16; ++t) {
+                    const uint32_t a[4] = {
+                        Num<T>::pack(s[2 * t][0], s[2 * t][1]), Num<T>::pack(s[2 * t][2], s[2 * t][3]),
+                        Num<T>::pack(s[2 * t + 1][0], s[2 * t + 1][1]), Num<T>::pack(s[2 * t + 1][2], s[2 * t + 1][3])};
+#pragma unroll
+                    for (int nn = 0; nn < D / 16; ++nn) {
+                        uint32_t f[4];
+                        ldsm4t(f, (vb ^ (nn << 5)) + t * 16 * kRow);
+                        Num<T>::mma(o[2 * nn], a, f[0], f[1]);
+                        Num<T>::mma(o[2 * nn + 1], a, f[2], f[3]);
+                    }
                 }
             }
         }
@@ -453,9 +505,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
                 }
             }
             if (to_end && warp == 0 && lane == 0) {
-                // the block with the item's first unit: the last one whose share begins at or before it
-                const int64_t first = ((item_u0 + 1) * workers - 1) / total;
-                p.span[item] = make_int2((int32_t)first, (int32_t)me);
+                p.span[item] = make_int2(shares.owner(item_u0), me);
             }
         }
         at.unit = at.units - 1;
@@ -464,110 +514,147 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
     cp_wait<0>();
 }
 
-// Joins the parts of items that were cut (blocks y < splits: each has 16 / slices of the output's 8-column tiles of one
-// 16-head tile, `slices` warps sharing a column's parts), and gathers weights (the others).  Blocks x: items.
+// Joins the parts of items that were cut (blocks y < splits: each has `tiles` of the output's 8-column tiles of one
+// 16-head tile, and slices = 16 / tiles warps share a tile's parts), and gathers weights (the other blocks y).  Blocks
+// x: items.  All of it is latency: every load of a thread that another does not need first is under way at once.
 template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p, int32_t slices, int32_t splits) {
-    constexpr int kJoinWarps = kJoinThreads / 32;
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p, int32_t tiles, int32_t splits) {
+    constexpr int kJoinWarps = kJoinThreads / 32, kMl = kMaxWorkers / 32, kBatch = 10;
     __shared__ float factor[kMaxWorkers][16];  // of each part and head: 2^(m - M) / L
     __shared__ float4 sums[kJoinWarps][32];
-    __shared__ float z[kMaxG];
+    __shared__ __align__(16) float z[kMaxG];
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t item = blockIdx.x;
-    const int32_t b = (int32_t)(item / p.Hk), g = (int32_t)(item % p.Hk);
+    const int32_t item = blockIdx.x, b = item / p.Hk, g = item - b * p.Hk;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int32_t len = length(p, b);
     const bool join = (int)blockIdx.y < splits;
+    const int2 sp = __ldcg(&p.span[item]);
     if (len == 0) {
         if (blockIdx.y == 0) {
-            uint32_t *op = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p.out) + item * p.G * D * 2);
+            uint32_t *op = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p.out) + (int64_t)item * p.G * D * 2);
             for (int i = tid; i < p.G * D / 2; i += kJoinThreads) op[i] = 0u;
             if (p.lse)
-                for (int i = tid; i < p.G; i += kJoinThreads) p.lse[item * p.G + i] = -INFINITY;
+                for (int i = tid; i < p.G; i += kJoinThreads) p.lse[(int64_t)item * p.G + i] = -INFINITY;
         }
         return;
     }
-    const int2 sp = __ldcg(&p.span[item]);
     const int32_t parts = sp.y - sp.x + 1;
     if (join && parts == 1) return;
     auto spot = [&](int32_t i) { return 2 * (int64_t)(sp.x + i) + (i == 0 ? 1 : 0); };
-    // M and L of each head: one warp a head
+    // M and L of each head of a tile: one warp a head
     auto stats = [&](int ht, bool factors) {
-        const int64_t row = ht * 16 + warp;
+        float2 v[kMl];
+#pragma unroll
+        for (int j = 0; j < kMl; ++j) {
+            const int32_t i = lane + 32 * j;
+            v[j] = make_float2(-INFINITY, 0.f);
+            if (32 * j < parts && i < parts) v[j] = __ldcg(&p.part_ml[spot(i) * (16 * MT) + ht * 16 + warp]);
+        }
         float M = -INFINITY, L = 0.f;
-        for (int32_t i = lane; i < parts; i += 32) M = fmaxf(M, __ldcg(&p.part_ml[spot(i) * (16 * MT) + row]).x);
+#pragma unroll
+        for (int j = 0; j < kMl; ++j) M = fmaxf(M, v[j].x);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
         const float base = M == -INFINITY ? 0.f : M;
-        for (int32_t i = lane; i < parts; i += 32) {
-            const float2 v = __ldcg(&p.part_ml[spot(i) * (16 * MT) + row]);
-            L += v.y * ex2(v.x - base);
+#pragma unroll
+        for (int j = 0; j < kMl; ++j) {
+            v[j].x = ex2(v[j].x - base);
+            L += v[j].y * v[j].x;
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
         if (factors) {
             const float inv = L != 0.f ? 1.f / L : 0.f;
-            for (int32_t i = lane; i < parts; i += 32)
-                factor[i][warp] = ex2(__ldcg(&p.part_ml[spot(i) * (16 * MT) + row]).x - base) * inv;
+#pragma unroll
+            for (int j = 0; j < kMl; ++j)
+                if (lane + 32 * j < parts) factor[lane + 32 * j][warp] = v[j].x * inv;
         }
         return L != 0.f ? M + log2f(L) : -INFINITY;
     };
     if (join) {
-        const int per = kJoinWarps / slices;              // 8-column tiles of this block
-        const int ht = blockIdx.y / (D / 8 / per), tile = blockIdx.y % (D / 8 / per) * per + warp / slices;
+        const int slices = kJoinWarps / tiles, per_ht = D / 8 / tiles;
+        const int ht = blockIdx.y / per_ht, tile = blockIdx.y % per_ht * tiles + warp / slices;
+        const float4 *src = p.part_o + (int64_t)(ht * (D / 8) + tile) * 32 + lane;
+        const int32_t i0 = warp % slices;
+        float4 v[kBatch];
+        auto load = [&](int32_t i) {
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j)
+                if (i + j * slices < parts) v[j] = __ldcg(src + spot(i + j * slices) * (MT * (D / 8) * 32));
+        };
+        load(i0);  // while M and L are found
         const float lse2 = stats(ht, true);
-        if (p.lse && blockIdx.y % (D / 8 / per) == 0 && lane == 0 && ht * 16 + warp < p.G)
-            p.lse[item * p.G + ht * 16 + warp] = lse2 * kLn2;
+        if (p.lse && blockIdx.y % per_ht == 0 && lane == 0 && ht * 16 + warp < p.G)
+            p.lse[(int64_t)item * p.G + ht * 16 + warp] = lse2 * kLn2;
         __syncthreads();
         const int r0 = lane >> 2;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int32_t i = warp % slices; i < parts; i += slices) {
-            const float4 v = __ldcg(&p.part_o[((spot(i) * MT + ht) * (D / 8) + tile) * 32 + lane]);
-            const float f0 = factor[i][r0], f1 = factor[i][r0 + 8];
-            acc.x += v.x * f0;
-            acc.y += v.y * f0;
-            acc.z += v.z * f1;
-            acc.w += v.w * f1;
+        for (int32_t i = i0; i < parts; i += kBatch * slices) {
+            if (i != i0) load(i);
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j)
+                if (i + j * slices < parts) {
+                    const float f0 = factor[i + j * slices][r0], f1 = factor[i + j * slices][r0 + 8];
+                    acc.x += v[j].x * f0;
+                    acc.y += v[j].y * f0;
+                    acc.z += v[j].z * f1;
+                    acc.w += v[j].w * f1;
+                }
         }
-        sums[warp][lane] = acc;
-        __syncthreads();
-        if (warp % slices == 0) {
+        if (slices > 1) {
+            sums[warp][lane] = acc;
+            __syncthreads();
+            if (i0) return;
             for (int i = 1; i < slices; ++i) {
-                const float4 v = sums[warp + i][lane];
-                acc.x += v.x;
-                acc.y += v.y;
-                acc.z += v.z;
-                acc.w += v.w;
+                const float4 y = sums[warp + i][lane];
+                acc.x += y.x;
+                acc.y += y.y;
+                acc.z += y.z;
+                acc.w += y.w;
             }
-            const int left = p.G - ht * 16;
-            uint32_t *op = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p.out) +
-                                                        ((item * p.G + ht * 16 + r0) * D + tile * 8 + (lane & 3) * 2) * 2);
-            if (r0 < left) op[0] = Num<T>::pack(acc.x, acc.y);
-            if (r0 + 8 < left) op[4 * D] = Num<T>::pack(acc.z, acc.w);
         }
+        const int left = p.G - ht * 16;
+        uint32_t *op = reinterpret_cast<uint32_t *>(
+            static_cast<uint8_t *>(p.out) + (((int64_t)item * p.G + ht * 16 + r0) * D + tile * 8 + (lane & 3) * 2) * 2);
+        if (r0 < left) op[0] = Num<T>::pack(acc.x, acc.y);
+        if (r0 + 8 < left) op[4 * D] = Num<T>::pack(acc.z, acc.w);
         return;
     }
+    // weights: four positions a thread
     if (parts == 1) {
-        if (tid < p.G) z[tid] = __ldcg(&p.lse2[item * (16 * MT) + tid]);
+        if (tid < p.G) z[tid] = __ldcg(&p.lse2[(int64_t)item * (16 * MT) + tid]);
     } else {
         for (int ht = 0; ht < MT; ++ht) {
             const float lse2 = stats(ht, false);
-            if (lane == 0 && ht * 16 + warp < p.G) z[ht * 16 + warp] = lse2;
+            if (lane == 0) z[ht * 16 + warp] = lse2;
         }
     }
     __syncthreads();
-    const float *sc = p.scores + item * p.G * p.score_ld;
+    const float *sc = p.scores + (int64_t)item * p.G * p.score_ld;
     float *w = p.weights + b * p.w_sb + g * p.w_sh;
     const int32_t n_blocks = gridDim.y - splits, mine = blockIdx.y - splits;
-    for (int64_t pos = (int64_t)mine * kJoinThreads + tid; pos < len; pos += (int64_t)n_blocks * kJoinThreads) {
-        float x = 0.f;
+    for (int64_t pos = 4 * ((int64_t)mine * kJoinThreads + tid); pos < len; pos += 4 * (int64_t)n_blocks * kJoinThreads) {
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        // positions not held have a score of -inf: they gather nothing, even where the head's lse is NaN
+        auto term = [](float s, float zh) { return s == -INFINITY || zh == -INFINITY ? 0.f : ex2(s - zh); };
+        const int32_t n = min(4, (int32_t)(len - pos));
+        float old[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < n) old[i] = w[pos + i];
 #pragma unroll 8
         for (int h = 0; h < p.G; ++h) {
-            const float s = __ldcs(sc + h * p.score_ld + pos);
-            x += s == -INFINITY || z[h] == -INFINITY ? 0.f : ex2(s - z[h]);  // positions not held have s = -inf
+            const float4 s = __ldcs(reinterpret_cast<const float4 *>(sc + h * p.score_ld + pos));
+            const float zh = z[h];
+            x.x += term(s.x, zh);
+            x.y += term(s.y, zh);
+            x.z += term(s.z, zh);
+            x.w += term(s.w, zh);
         }
-        w[pos] += x;
+        const float add[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < n) w[pos + i] = old[i] + add[i];
     }
 }
 
@@ -604,25 +691,20 @@ Layout layout_of(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t max_len, 
 }
 
 template <typename T, int D, int MT> int launch(const Params &p, cudaStream_t s) {
-    constexpr int kTeams = kWarps / MT;
-    constexpr uint32_t kSlot = 2 * kStep * D * 2;
-    constexpr uint32_t kSlots = kRingBytes / (kTeams * kSlot) > 8 ? 8 : kRingBytes / (kTeams * kSlot);
-    constexpr uint32_t smem = kTeams * kSlots * kSlot + (kTeams > 1 ? 2 * (D / 8) * 32 * 16 : 0);
+    constexpr uint32_t smem = Shape<D, MT>::kSmem;
     UNUM_CHECK_CUDA(cudaFuncSetAttribute(attend_kernel<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     attend_kernel<T, D, MT><<<(unsigned)p.workers, kThreads, smem, s>>>(p);
     if (int rc = unum::check_launch("attend_kernel")) return rc;
     const int64_t items = (int64_t)p.B * p.Hk;
-    // Parts an item has at most: that many blocks share the whole work.  `slices` warps share a column's parts.
-    int slices = 1;
-    while (slices < 16 && slices * 4 * items < p.workers) slices *= 2;
-    int tiles = D / 8;  // of a block: all its warps on one slice, at most
-    if (16 / slices < tiles) tiles = 16 / slices;
-    slices = 16 / tiles;
+    // A long item is cut into about workers / items parts, and then a block of the second kernel has one tile's columns
+    // and 16 warps on its parts; where items are many they have a few parts each, and a block has the whole row.
+    int tiles = D / 8;
+    while (tiles > 1 && 16 / tiles * 4 * items < p.workers) tiles /= 2;
     const int splits = MT * (D / 8) / tiles;
     int64_t gather = 0;
     if (p.weights) {
         gather = (4 * (int64_t)p.workers + items - 1) / items;
-        const int64_t most = ((int64_t)p.max_len + kJoinThreads - 1) / kJoinThreads;
+        const int64_t most = ((int64_t)p.max_len + 4 * kJoinThreads - 1) / (4 * kJoinThreads);
         if (gather > most) gather = most;
     }
     cudaLaunchConfig_t cfg = {};
@@ -634,7 +716,7 @@ template <typename T, int D, int MT> int launch(const Params &p, cudaStream_t s)
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    UNUM_CHECK_CUDA(cudaLaunchKernelEx(&cfg, join_kernel<T, D, MT>, p, (int32_t)slices, (int32_t)splits));
+    UNUM_CHECK_CUDA(cudaLaunchKernelEx(&cfg, join_kernel<T, D, MT>, p, (int32_t)tiles, (int32_t)splits));
     return unum::check_launch("join_kernel");
 }
 
@@ -680,7 +762,11 @@ extern "C" int unum_paged_attention(const void *q, int64_t B, int64_t Hq, int64_
                    "q, k_cache, v_cache and out must be 16-byte aligned");
     UNUM_CHECK_ARG((q_sb | q_sh | k_st | k_sh | v_st | v_sh) % 8 == 0,
                    "strides of q, k_cache and v_cache must be multiples of 8 elements");
-    UNUM_CHECK_ARG(B < ((int64_t)1 << 31) / Hk && Hk < 65536, "too many sequences or kv heads");
+    UNUM_CHECK_ARG(k_st >= 0 && k_st < (1 << 30) && v_st >= 0 && v_st < (1 << 30),
+                   "token strides of k_cache and v_cache must be below 2^30 elements");
+    UNUM_CHECK_ARG(Hk < 65536 && B < ((int64_t)1 << 31) / Hk &&
+                       B * Hk < ((int64_t)1 << 31) / ((max_seqlen + kUnit - 1) / kUnit + 1),
+                   "too many sequences, kv heads or positions");
     UNUM_CHECK_ARG(max_seqlen <= ((int64_t)1 << 31) - 2 * kUnit && n_tokens < ((int64_t)1 << 31),
                    "max_seqlen and n_tokens must stay below 2^31");
     const Layout l = layout_of(B, Hq, Hk, D, max_seqlen, weights != nullptr);
@@ -691,7 +777,8 @@ extern "C" int unum_paged_attention(const void *q, int64_t B, int64_t Hq, int64_
     }
     Params p;
     p.q = (const uint8_t *)q, p.kc = (const uint8_t *)k_cache, p.vc = (const uint8_t *)v_cache;
-    p.q_sb = 2 * q_sb, p.q_sh = 2 * q_sh, p.k_st = 2 * k_st, p.k_sh = 2 * k_sh, p.v_st = 2 * v_st, p.v_sh = 2 * v_sh;
+    p.q_sb = 2 * q_sb, p.q_sh = 2 * q_sh, p.k_sh = 2 * k_sh, p.v_sh = 2 * v_sh;
+    p.k_st = (int32_t)(2 * k_st), p.v_st = (int32_t)(2 * v_st);
     p.table = block_table;
     p.lens = seqlens;
     p.bt_stride = bt_stride;
