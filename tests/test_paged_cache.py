@@ -475,7 +475,8 @@ EVICT = [
     ([1000, 999], 2, 1, 300, 0, 1, "ties"), ([1000, 40], 3, 16, 20, 1, 2, "random"), ([513, 77], 1, 2, 100, 0, 7, "ties"),
     ([4000, 4096, 1], 2, 64, 9, 1, 2, "random"), ([300], 2, 1, 10, 4, 6, "random"), ([20000, 3], 2, 1, 5000, 10, 100, "random"),
     ([2048], 2, 1, 1024, 0, 1, "equal"), ([700], 2, 4, 50, 2, 2, "odd"), ([150000], 1, 1, 70000, 5, 9, "random"),
-    ([9000], 2, 256, 7, 0, 1, "negative"), ([50] * 30, 2, 8, 3, 1, 1, "ties"), ([33] * 5, 4, 32, 1, 0, 1, "random"),
+    ([9000], 2, 256, 7, 0, 1, "negative"), ([50] * 30, 2, 8, 3, 1, 1, "ties"),
+    ([409598], 1, 1, 300001, 3, 1, "random"), ([120000, 90000, 5], 2, 1, 60000, 3, 1, "ties"), ([33] * 5, 4, 32, 1, 0, 1, "random"),
 ]
 
 

@@ -51,14 +51,24 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
 // ------------------------------------------------------------------------------------------------ evict
 // One cluster of C blocks for each sequence; block r has a contiguous slice of its pages in use, with one 32-bit key
 // a page in shared memory (the float's bits in an order that compares as unsigned; 0 = NaN).
-//   keys     the sums, and the histogram of the keys' top digit;
-//   select   radix selection over four 8-bit digits: every block adds up the cluster's histograms through distributed
-//            shared memory and takes the same decision, one cluster barrier a digit;
-//   write    a scan over the slice gives each page its place, among those that stay or among the evicted; the list of
-//            the pages that stay takes the keys' room, and the weights move along it.
-constexpr int kEvThreads = 1024;
-constexpr int kMaxCluster = 8;
-constexpr int64_t kMaxSlice = 51200;  // 4 bytes a page: 200 KB of shared memory
+//   keys     the sums, four pages a thread (or group of threads) under way at once;
+//   select   radix selection over four 8-bit digits.  Keys crowd into few bins of the first, so a block counts in eight
+//            histograms by lane.  After a cluster barrier every block adds up the cluster's counts through distributed
+//            shared memory and takes the same decision.  (Adding them up with remote atomics took 13 us a digit with 16
+//            blocks: they are served one at a time.)
+//   write    each warp has a contiguous part of the slice; a count and one scan over the warps give each page its
+//            place, among those that stay or among the evicted, and the weights move along, 128 pages at a time.
+// What is filled behind the new ends does not wait for any of it and is written first.
+// Bound by latency for one sequence (the barriers), by HBM for a batch.
+constexpr int kEvThreads = 512;  // with 1024, block barriers cost more than the added warps hid (12.5 against 10.3 us)
+constexpr int kEvWarps = kEvThreads / 32;
+constexpr int kMaxCluster = 16;
+constexpr int64_t kMaxSlice = 25600;  // 4 bytes a page: 100 KB of shared memory
+constexpr int64_t kMaxPages = kMaxCluster * kMaxSlice;
+constexpr int kBins = 256;
+constexpr int kGroups = kEvThreads / kBins;
+constexpr int kCopies = 8;   // of the histogram
+constexpr int kBatch = 4;    // loads of a thread under way, and 32-page chunks of a warp's write step
 
 struct EvictParams {
     const int32_t *table, *seqlens;
@@ -98,43 +108,39 @@ __device__ __forceinline__ void cluster_barrier() {
     cluster_wait();
 }
 
-// A 32-bit word of another block's shared memory.
-__device__ __forceinline__ uint32_t ld_cluster(const void *mine, uint32_t rank) {
-    uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(mine)), v;
-    asm volatile("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(a) : "r"(rank));
+// The address of this block's shared memory location in block `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer(const void *mine, uint32_t rank) {
+    uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(mine)), r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t ld_cluster(uint32_t a) {
+    uint32_t v;
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
     return v;
 }
 
-// Exclusive scan of one value a thread over the block, and the block's total.
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *warp_sums, uint32_t &total) {
+// Exclusive scan over the block's warps of a value that each warp's lanes agree on, and the total.
+__device__ __forceinline__ uint32_t scan_warps(uint32_t v, uint32_t *warp_sums, uint32_t &total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint32_t x = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-    }
-    if (lane == 31) warp_sums[warp] = x;
+    __syncthreads();  // warp_sums may still be read
+    if (lane == 0) warp_sums[warp] = v;
     __syncthreads();
-    uint32_t s = warp_sums[lane];  // 32 warps
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += y;
-    }
-    total = __shfl_sync(0xffffffffu, s, 31);
-    const uint32_t before = __shfl_sync(0xffffffffu, s, (warp + 31) & 31);
-    __syncthreads();  // warp_sums is used again
-    return x - v + (warp ? before : 0);
+    const uint32_t x = lane < kEvWarps ? warp_sums[lane] : 0;
+    total = __reduce_add_sync(0xffffffffu, x);
+    return __reduce_add_sync(0xffffffffu, lane < warp ? x : 0);
 }
 
-__global__ void __launch_bounds__(kEvThreads, 1) evict_kernel(const __grid_constant__ EvictParams p) {
-    extern __shared__ uint32_t keys[];  // this block's slice; later the list of pages that stay
-    __shared__ uint32_t hist[4][256], all[256];
-    __shared__ uint32_t warp_sums[32];
+// kVec: pages of 4 positions and more whose weights 16-byte loads can read.
+template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kernel(const __grid_constant__ EvictParams p) {
+    extern __shared__ uint32_t keys[];  // this block's slice
+    __shared__ uint32_t hist[kCopies][kBins], counts[4][kBins];  // counts: this block's, of each digit
+    __shared__ uint32_t sums[kGroups][kBins];                    // the cluster's, of every kGroups-th block
+    __shared__ uint32_t warp_sums[kEvWarps];
     __shared__ uint32_t found[2];    // the digit, and how many are still wanted inside it
-    __shared__ uint32_t slice_kept;
+    __shared__ uint32_t slice_eq, slice_sure;
+    __shared__ int32_t list[kEvWarps][32 * kBatch];  // of a warp's pages in hand those that stay
     const uint32_t rank = cluster_rank(), C = cluster_size();
     const int64_t b = blockIdx.x / C;
     const int32_t P = 1 << p.shift;
@@ -142,67 +148,141 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_kernel(const __grid_const
     len = len < 0 ? 0 : (len > p.n_pages * P ? p.n_pages * P : len);
     const int64_t used = (len + P - 1) >> p.shift;
     const int64_t drop = used > p.budget ? used - p.budget : 0;
-    const int64_t cand0 = p.init, cand1 = used - p.local;  // the pages that may go (only where drop > 0)
     const int64_t per = (used + C - 1) / C;
     const int64_t s0 = per * rank < used ? per * rank : used;
     const int64_t s1 = s0 + per < used ? s0 + per : used;
     const int32_t n = (int32_t)(s1 - s0);
+    // the pages that may go (only where drop > 0), within the slice
+    const int64_t c0 = p.init - s0, c1 = used - p.local - s0;
+    const int32_t cand0 = (int32_t)(c0 < 0 ? 0 : (c0 > n ? n : c0)), cand1 = (int32_t)(c1 < 0 ? 0 : (c1 > n ? n : c1));
     const float *wb = p.w + b * p.w_sb;
     float *nwb = p.new_w + b * (int64_t)p.Hk * p.W;
     const int32_t *trow = p.table + b * p.bt_stride;
     int32_t *nrow = p.new_table + b * p.n_pages, *erow = p.evicted + b * p.n_pages;
-    const int tid = threadIdx.x, lane = tid & 31;
-    int64_t kept_before = s0;  // pages that stay, of the slices before this one
-    int32_t kept = n;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // a warp's part of the slice
+    const int32_t part = ((n + kEvWarps - 1) / kEvWarps + 31) / 32 * 32;
+    const int32_t i0 = min(warp * part, n), i1 = min(i0 + part, n);
+    // pages that stay: of the slices before this one, and of this slice before the warp's part
+    int64_t kept_before = s0;
+    uint32_t stay_at = i0;
+    uint32_t edge = 0, eq_at = 0, eq_left = 0;  // the lightest key that stays; pages of it so far, and those that may stay
+
+    // behind what stays: pages of the row that are not in use yet move up, and nothing fills the rest
+    const int64_t me = (int64_t)rank * kEvThreads + tid, all_threads = (int64_t)C * kEvThreads;
+    for (int64_t e = used + me; e < p.n_pages; e += all_threads) nrow[e - drop] = __ldg(trow + e);
+    for (int64_t e = me; e < drop; e += all_threads) nrow[p.n_pages - drop + e] = -1;
+    for (int64_t e = drop + me; e < p.n_pages; e += all_threads) erow[e] = -1;
+    const int64_t end = (used - drop) << p.shift;
+    if (p.W % 4 == 0) {
+        const int64_t end4 = (end + 3) / 4 * 4;
+        for (int32_t h = 0; h < p.Hk; ++h) {
+            float *row = nwb + h * p.W;
+            for (int64_t j = end4 + 4 * me; j < p.W; j += 4 * all_threads)
+                *reinterpret_cast<float4 *>(row + j) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (me < end4 - end) row[end + me] = 0.0f;
+        }
+    } else {
+        for (int32_t h = 0; h < p.Hk; ++h)
+            for (int64_t j = end + me; j < p.W; j += all_threads) nwb[h * p.W + j] = 0.0f;
+    }
 
     if (drop > 0) {
-        for (int i = tid; i < 4 * 256; i += kEvThreads) (&hist[0][0])[i] = 0;
+        for (int i = tid; i < kCopies * kBins; i += kEvThreads) (&hist[0][0])[i] = 0;
         __syncthreads();
-        // keys; `per_page` lanes share a page
-        const int per_page = P < 32 ? P : 32;
-        const int sub = tid & (per_page - 1);
-        for (int32_t i0 = 0; i0 < n; i0 += kEvThreads / per_page) {
-            const int32_t i = i0 + tid / per_page;
-            double sum = 0.0;
-            if (i < n) {
-                const int64_t at = (s0 + i) << p.shift;
-                for (int32_t h = 0; h < p.Hk; ++h)
-                    for (int32_t j = sub; j < P; j += per_page)
-                        if (at + j < len) sum += (double)__ldg(wb + h * p.w_sh + at + j);
+        // keys; `lanes` threads share a page
+        constexpr int kWide = kVec ? 4 : 1;
+        const int lanes = P < 32 * kWide ? P / kWide : 32;
+        const int sub = (tid & (lanes - 1)) * kWide;
+        const int32_t stride = kEvThreads / lanes;
+        uint32_t *my_hist = hist[lane & (kCopies - 1)];
+        if (lanes >= kCopies) my_hist = hist[(tid / lanes) & (kCopies - 1)];
+        for (int32_t i00 = tid / lanes; i00 < n + tid / lanes; i00 += kBatch * stride) {
+            double sum[kBatch] = {};
+            for (int32_t j = sub; j < P; j += lanes * kWide) {
+#pragma unroll 2
+                for (int32_t h = 0; h < p.Hk; ++h) {
+                    const float *src = wb + h * p.w_sh + (s0 << p.shift) + j;
+                    if (kVec) {
+                        float4 v[kBatch];
+#pragma unroll
+                        for (int e = 0; e < kBatch; ++e)
+                            if (i00 + e * stride < n)
+                                v[e] = __ldg(reinterpret_cast<const float4 *>(src + ((int64_t)(i00 + e * stride) << p.shift)));
+#pragma unroll
+                        for (int e = 0; e < kBatch; ++e) {
+                            const int64_t left = len - ((s0 + i00 + e * stride) << p.shift) - j;
+                            if (left >= 4) {
+                                sum[e] += ((double)v[e].x + (double)v[e].y) + ((double)v[e].z + (double)v[e].w);
+                            } else {
+                                if (left > 0) sum[e] += (double)v[e].x;
+                                if (left > 1) sum[e] += (double)v[e].y;
+                                if (left > 2) sum[e] += (double)v[e].z;
+                            }
+                        }
+                    } else {
+                        float v[kBatch];
+#pragma unroll
+                        for (int e = 0; e < kBatch; ++e) {
+                            const int64_t at = ((int64_t)(i00 + e * stride) << p.shift);
+                            v[e] = i00 + e * stride < n && (s0 << p.shift) + at + j < len ? __ldg(src + at) : 0.0f;
+                        }
+#pragma unroll
+                        for (int e = 0; e < kBatch; ++e) sum[e] += (double)v[e];
+                    }
+                }
             }
-            for (int o = per_page >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (i < n && sub == 0) {
-                const uint32_t key = order_key((float)sum);
-                keys[i] = key;
-                if (s0 + i >= cand0 && s0 + i < cand1) atomicAdd(&hist[0][key >> 24], 1u);
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) {
+                for (int o = lanes >> 1; o > 0; o >>= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], o);
+                const int32_t i = i00 + e * stride;
+                if (i < n && sub == 0) {
+                    const uint32_t key = order_key((float)sum[e]);
+                    keys[i] = key;
+                    if (i >= cand0 && i < cand1) atomicAdd(&my_hist[key >> 24], 1u);
+                }
             }
         }
         // the key of the lightest page that stays, digit by digit
         uint32_t prefix = 0;
-        uint32_t want = (uint32_t)(cand1 - cand0 - drop);  // candidates that stay
+        uint32_t want = (uint32_t)(p.budget - p.init - p.local);  // candidates that stay
         const bool any = want > 0;
+        my_hist = hist[lane & (kCopies - 1)];
         for (int d = 0; d < 4 && any; ++d) {
             const int sh = 24 - 8 * d;
             if (d > 0) {
-                __syncthreads();
-                for (int32_t i = tid; i < n; i += kEvThreads) {
+#pragma unroll 4
+                for (int32_t i = cand0 + tid; i < cand1; i += kEvThreads) {
                     const uint32_t key = keys[i];
-                    if ((key >> (sh + 8)) == prefix && s0 + i >= cand0 && s0 + i < cand1)
-                        atomicAdd(&hist[d][(key >> sh) & 255u], 1u);
+                    if ((key >> (sh + 8)) == prefix) atomicAdd(&my_hist[(key >> sh) & 255u], 1u);
                 }
             }
-            cluster_barrier();
-            if (tid < 256) {
+            __syncthreads();
+            if (tid < kBins) {
                 uint32_t c = 0;
-                for (uint32_t r = 0; r < C; ++r) c += ld_cluster(&hist[d][tid], r);
-                all[tid] = c;
+#pragma unroll
+                for (int i = 0; i < kCopies; ++i) {
+                    c += hist[i][tid];
+                    hist[i][tid] = 0;
+                }
+                counts[d][tid] = c;
+            }
+            if (C > 1) cluster_barrier();
+            else __syncthreads();
+            {
+                uint32_t c = 0;
+#pragma unroll 8
+                for (uint32_t r = tid / kBins; r < C; r += kGroups) c += C > 1 ? ld_cluster(peer(&counts[d][tid % kBins], r)) : counts[d][tid % kBins];
+                sums[tid / kBins][tid % kBins] = c;
             }
             __syncthreads();
-            if (tid < 32) {  // lane l has digits 255 - 8l .. 248 - 8l: a scan from the top
+            if (warp == 0) {  // lane l has digits 255 - 8l .. 248 - 8l: a scan from the top
                 uint32_t c[8], sum = 0;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    c[e] = all[255 - 8 * lane - e];
+                    c[e] = 0;
+#pragma unroll
+                    for (int i = 0; i < kGroups; ++i) c[e] += sums[i][255 - 8 * lane - e];
                     sum += c[e];
                 }
                 uint32_t above = sum;
@@ -225,75 +305,111 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_kernel(const __grid_const
             prefix = (prefix << 8) | found[0];
             want = found[1];
         }
-        // pages of exactly that key: `want` of them stay, the first ones
-        uint32_t eq_left = 0, eq_here = 0;
-        if (any) {
-            uint32_t eq_before = 0;
-            for (uint32_t r = 0; r < rank; ++r) eq_before += ld_cluster(&hist[3][prefix & 255u], r);
-            eq_here = hist[3][prefix & 255u];
-            eq_left = want > eq_before ? want - eq_before : 0;
-            eq_left = eq_left < eq_here ? eq_left : eq_here;
+        // Of the pages of exactly that key the first `want` stay.  What this warp's part has of them, and of what stays
+        // for sure:
+        uint32_t n_sure = 0, n_eq = 0;
+        for (int32_t i = i0 + lane; i < i1; i += 32) {
+            const uint32_t key = keys[i];
+            const bool s = i < cand0 || i >= cand1 || (any && key > prefix);
+            n_sure += s;
+            n_eq += !s && any && key == prefix;
         }
-        auto sure = [&](int32_t i) {
-            const int64_t e = s0 + i;
-            return e < cand0 || e >= cand1 || (any && keys[i] > prefix);
-        };
-        uint32_t n_sure = 0;
-        for (int32_t i = tid; i < n; i += kEvThreads) n_sure += sure(i);
-        uint32_t total;
-        block_scan(n_sure, warp_sums, total);
-        if (tid == 0) slice_kept = total + eq_left;
-        kept = (int32_t)(total + eq_left);
-        cluster_barrier();
-        kept_before = 0;
-        for (uint32_t r = 0; r < rank; ++r) kept_before += ld_cluster(&slice_kept, r);
-        cluster_arrive();  // waited for at the end: no block leaves while another reads its shared memory
-        // places: among those that stay, or among the evicted
-        uint32_t base = 0, eq_base = 0;
-        for (int32_t i0 = 0; i0 < n; i0 += kEvThreads) {
-            const int32_t i = i0 + tid;
-            const bool is_sure = i < n && sure(i);
-            const bool eq = i < n && !is_sure && any && keys[i] == prefix;
-            uint32_t n_eq, n_stay;
-            const uint32_t eq_at = block_scan(eq ? 1u : 0u, warp_sums, n_eq) + eq_base;
-            const bool stay = is_sure || (eq && eq_at < eq_left);
-            const uint32_t at = block_scan(stay ? 1u : 0u, warp_sums, n_stay) + base;
-            if (i < n) {
-                const int32_t page = __ldg(trow + s0 + i);
-                if (stay) {
-                    keys[at] = (uint32_t)i;  // at <= i: this chunk's keys have been read
-                    nrow[kept_before + at] = page;
+        n_sure = __reduce_add_sync(0xffffffffu, n_sure);
+        n_eq = __reduce_add_sync(0xffffffffu, n_eq);
+        uint32_t all_sure, all_eq;
+        const uint32_t sure_at = scan_warps(n_sure, warp_sums, all_sure);
+        eq_at = scan_warps(n_eq, warp_sums, all_eq);
+        if (tid == 0) {
+            slice_eq = all_eq;
+            slice_sure = all_sure;
+        }
+        if (C > 1) cluster_barrier();
+        // slices before this one: their pages of that key come first
+        uint32_t eq_before = 0, sure_before = 0;
+        for (uint32_t r = 0; r < rank; ++r) {
+            eq_before += ld_cluster(peer(&slice_eq, r));
+            sure_before += ld_cluster(peer(&slice_sure, r));
+        }
+        if (C > 1) cluster_arrive();  // waited for at the end: no block leaves while another reads its shared memory
+        if (!any) want = 0;
+        eq_left = want - min(eq_before, want);  // of this slice's, the first ones
+        kept_before = sure_before + min(eq_before, want);
+        stay_at = sure_at + min(eq_at, eq_left);
+        edge = any ? prefix : 0xffffffffu;
+    }
+    // places, and the weights of the pages that stay
+    for (int32_t j0 = i0; j0 < i1; j0 += 32 * kBatch) {
+        const uint32_t below = (1u << lane) - 1;
+        int32_t page[kBatch], m = 0;
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e)
+            if (j0 + 32 * e + lane < i1) page[e] = __ldg(trow + s0 + j0 + 32 * e + lane);
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+            const int32_t i = j0 + 32 * e + lane;
+            bool stay = i < i1;
+            if (drop > 0) {
+                const uint32_t key = stay ? keys[i] : 0;
+                const bool sure = stay && (i < cand0 || i >= cand1 || key > edge);
+                const bool eq = stay && !sure && key == edge;
+                const uint32_t eqs = __ballot_sync(0xffffffffu, eq);
+                stay = sure || (eq && eq_at + __popc(eqs & below) < eq_left);
+                eq_at += __popc(eqs);
+            }
+            const uint32_t stays = __ballot_sync(0xffffffffu, stay);
+            const int32_t at = m + __popc(stays & below);
+            if (stay) {
+                nrow[kept_before + stay_at + at] = page[e];
+                list[warp][at] = i;
+            } else if (i < i1) {
+                erow[s0 + i - kept_before - stay_at - at] = page[e];
+            }
+            m += __popc(stays);
+        }
+        __syncwarp();
+        const int64_t to = (kept_before + stay_at) << p.shift;
+        stay_at += m;
+        m <<= p.shift;
+        constexpr int kWide = kVec ? 4 : 1;
+        for (int32_t q0 = lane * kWide; q0 < m; q0 += 32 * kWide * kBatch) {
+            int64_t from[kBatch];
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) {
+                const int32_t q = q0 + 32 * kWide * e;
+                from[e] = q < m ? ((s0 + list[warp][q >> p.shift]) << p.shift) + (q & (P - 1)) : len;
+            }
+#pragma unroll 2
+            for (int32_t h = 0; h < p.Hk; ++h) {
+                const float *src = wb + h * p.w_sh;
+                float *dst = nwb + h * p.W + to + q0;
+                if (kVec) {
+                    float4 v[kBatch];
+#pragma unroll
+                    for (int e = 0; e < kBatch; ++e)
+                        v[e] = from[e] < len ? __ldg(reinterpret_cast<const float4 *>(src + from[e]))
+                                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                    for (int e = 0; e < kBatch; ++e) {
+                        // behind the length: zero, whatever is there
+                        if (from[e] + 1 >= len) v[e].y = 0.0f;
+                        if (from[e] + 2 >= len) v[e].z = 0.0f;
+                        if (from[e] + 3 >= len) v[e].w = 0.0f;
+                        if (q0 + 128 * e < m) *reinterpret_cast<float4 *>(dst + 128 * e) = v[e];
+                    }
                 } else {
-                    erow[s0 - kept_before + i - at] = page;
+                    float v[kBatch];
+#pragma unroll
+                    for (int e = 0; e < kBatch; ++e) v[e] = from[e] < len ? __ldg(src + from[e]) : 0.0f;
+#pragma unroll
+                    for (int e = 0; e < kBatch; ++e)
+                        if (q0 + 32 * e < m) dst[32 * e] = v[e];
                 }
             }
-            base += n_stay;
-            eq_base += n_eq;
         }
-        __syncthreads();
-    } else {
-        for (int32_t i = tid; i < n; i += kEvThreads) {
-            keys[i] = (uint32_t)i;
-            nrow[s0 + i] = __ldg(trow + s0 + i);
-        }
-        __syncthreads();
+        __syncwarp();
     }
-    // the weights of the pages that stay
-    const int64_t m = (int64_t)kept << p.shift;
-    for (int64_t j = tid; j < m; j += kEvThreads) {
-        const int64_t at = ((s0 + keys[j >> p.shift]) << p.shift) + (j & (P - 1));
-        float *dst = nwb + (kept_before << p.shift) + j;
-        for (int32_t h = 0; h < p.Hk; ++h) dst[h * p.W] = at < len ? __ldg(wb + h * p.w_sh + at) : 0.0f;
-    }
-    // behind them: pages of the row that are not in use yet move up, and nothing fills the rest
-    const int64_t me = (int64_t)rank * kEvThreads + tid, all_threads = (int64_t)C * kEvThreads;
-    for (int64_t e = used + me; e < p.n_pages; e += all_threads) nrow[e - drop] = __ldg(trow + e);
-    for (int64_t e = me; e < drop; e += all_threads) nrow[p.n_pages - drop + e] = -1;
-    for (int64_t e = drop + me; e < p.n_pages; e += all_threads) erow[e] = -1;
-    for (int64_t j = ((used - drop) << p.shift) + me; j < p.W; j += all_threads)
-        for (int32_t h = 0; h < p.Hk; ++h) nwb[h * p.W + j] = 0.0f;
     if (rank == 0 && tid == 0) p.new_lens[b] = (int32_t)(len - (drop << p.shift));
-    if (drop > 0) cluster_wait();
+    if (drop > 0 && C > 1) cluster_wait();
 }
 
 bool power_of_two(int64_t x) { return x > 0 && (x & (x - 1)) == 0; }
@@ -367,9 +483,8 @@ extern "C" int unum_cache_evict(const int32_t *block_table, int64_t B, int64_t n
                    "budget must hold init_pages + local_pages (got %lld < %lld + %lld)", (long long)budget,
                    (long long)init_pages, (long long)local_pages);
     if (B == 0) return UNUM_OK;
-    if (n_pages > kMaxCluster * kMaxSlice) {
-        unum::set_error("at most %lld pages a sequence (got %lld)", (long long)(kMaxCluster * kMaxSlice),
-                        (long long)n_pages);
+    if (n_pages > kMaxPages) {
+        unum::set_error("at most %lld pages a sequence (got %lld)", (long long)kMaxPages, (long long)n_pages);
         return UNUM_ERR_UNSUPPORTED;
     }
     UNUM_CHECK_ARG(n_pages * page_size < ((int64_t)1 << 31), "n_pages * page_size must stay below 2^31");
@@ -377,6 +492,7 @@ extern "C" int unum_cache_evict(const int32_t *block_table, int64_t B, int64_t n
     UNUM_CHECK_ARG(seqlens && new_seqlens, "null pointer argument");
     UNUM_CHECK_ARG(n_pages == 0 || (block_table && weights && new_table && new_weights && evicted),
                    "null pointer argument");
+    UNUM_CHECK_ARG(unum::aligned16(new_weights), "new_weights must be 16-byte aligned");
     EvictParams p;
     p.table = block_table;
     p.seqlens = seqlens;
@@ -395,12 +511,17 @@ extern "C" int unum_cache_evict(const int32_t *block_table, int64_t B, int64_t n
     p.new_lens = new_seqlens;
     p.evicted = evicted;
     p.new_w = new_weights;
-    int C = 1;
-    while (C < kMaxCluster && n_pages > C * kMaxSlice) C *= 2;
+    // As many blocks a sequence as keep the whole batch resident (two an SM), while each still has 4096 weights or more.
+    int64_t C = 1;
+    while (C < kMaxCluster && (n_pages > C * kMaxSlice || (B * C * 2 <= 2 * unum::sm_count() &&
+                                                           n_pages * page_size * Hk >= C * 2 * 4096)))
+        C *= 2;
     const int64_t slice = (n_pages + C - 1) / C;
     const size_t smem = (size_t)(slice < 1 ? 1 : slice) * 4;
-    UNUM_CHECK_CUDA(cudaFuncSetAttribute(evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)(kMaxSlice * 4)));
+    const bool vec = page_size >= 4 && (w_sb | w_sh) % 4 == 0 && unum::aligned16(weights);
+    auto *kernel = vec ? evict_kernel<true> : evict_kernel<false>;
+    UNUM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kMaxSlice * 4)));
+    UNUM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(B * C));
     cfg.blockDim = dim3(kEvThreads);
@@ -412,6 +533,6 @@ extern "C" int unum_cache_evict(const int32_t *block_table, int64_t B, int64_t n
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    UNUM_CHECK_CUDA(cudaLaunchKernelEx(&cfg, evict_kernel, p));
+    UNUM_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
     return unum::check_launch("evict_kernel");
 }
