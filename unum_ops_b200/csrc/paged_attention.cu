@@ -38,9 +38,11 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kBlocksPerSm = 2;
 constexpr int kUnit = 64;            // positions dealt to a block at a time
 constexpr int kGrain = 2;            // units a block takes at least: below it the join costs more than the split gains
-constexpr int kMaxWorkers = 512;     // resident blocks, at most
+constexpr int kMaxWorkers = 296;     // resident blocks, at most: two on each of 148 SMs
 constexpr uint32_t kRingBytes = 96 * 1024;
 constexpr int kMaxG = 64;
+constexpr int kMaxCluster = 8;
+constexpr int kNearUnits = 8;        // of a cluster's block, at most (at head dim 128)
 constexpr int kJoinThreads = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -89,6 +91,42 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
 __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+
+__device__ __forceinline__ int32_t cluster_size() {
+    int32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ int32_t cluster_rank() {
+    int32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_arrive() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_barrier() {
+    cluster_arrive();
+    cluster_wait();
+}
+// The address of this block's shared memory location in block `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer(const void *mine, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(mine)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t a) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t a) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+    return v;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -177,6 +215,7 @@ __device__ __forceinline__ int32_t scan_units(const Params &p, int32_t b0, int32
 // The units are dealt out in a row: the first `more` blocks have base + 1 of them, the others base.
 struct Shares {
     int32_t base, more;
+    __device__ __forceinline__ Shares() {}
     __device__ __forceinline__ Shares(int32_t total, int32_t workers) : base(total / workers), more(total % workers) {}
     __device__ __forceinline__ int32_t begin(int32_t w) const { return w * base + min(w, more); }
     __device__ __forceinline__ int32_t owner(int32_t u) const {
@@ -184,6 +223,131 @@ struct Shares {
         return u < edge ? u / (base + 1) : more + (u - edge) / base;
     }
 };
+
+template <int D> __device__ __forceinline__ void write_empty(const Params &p, int64_t item, int threads) {
+    uint32_t *op = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p.out) + item * p.G * D * 2);
+    for (int i = threadIdx.x; i < p.G * D / 2; i += threads) op[i] = 0u;
+    if (p.lse)
+        for (int i = threadIdx.x; i < p.G; i += threads) p.lse[item * p.G + i] = -INFINITY;
+}
+
+// The weights that four positions from `pos` on gather from all heads of an item; z: the heads' lse in base 2.
+__device__ __forceinline__ void gather4(const Params &p, int64_t item, const float *z, float *w, int32_t pos, int32_t end) {
+    const float *sc = p.scores + item * p.G * p.score_ld + pos;
+    // positions not held have a score of -inf: they gather nothing, even where the head's lse is NaN
+    auto term = [](float s, float zh) { return s == -INFINITY || zh == -INFINITY ? 0.f : ex2(s - zh); };
+    float old[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (pos + i < end) old[i] = w[pos + i];
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int h = 0; h < p.G; ++h) {
+        const float4 s = __ldcs(reinterpret_cast<const float4 *>(sc + h * p.score_ld));
+        const float zh = z[h];
+        x.x += term(s.x, zh);
+        x.y += term(s.y, zh);
+        x.z += term(s.z, zh);
+        x.w += term(s.w, zh);
+    }
+    const float add[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (pos + i < end) w[pos + i] = old[i] + add[i];
+}
+
+// The end of an item that a cluster has: each block's first team leaves its output, maxima and sums (ml: of rows r0 and
+// r0 + 8) in shared memory, each block joins some of the 8-column tiles, in the order of the positions, and gathers the
+// weights of its own positions.
+template <typename T, int D, int MT>
+__device__ __forceinline__ void join_cluster(const Params &p, const float (&o)[D / 8][4], float2 ml0, float2 ml1, int64_t item,
+                                             int32_t C, int32_t rank, int32_t u0, int32_t u1, int32_t len, uint8_t *smem) {
+    __shared__ float2 ml[16 * MT];
+    __shared__ float z[16 * MT];
+    constexpr int kTiles = D / 8;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r0 = lane >> 2;
+    float4 *box = reinterpret_cast<float4 *>(smem);  // [MT][kTiles][32], where the ring was
+    cp_wait<0>();
+    __syncthreads();
+    if (warp < MT) {  // the first team
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i)
+            box[(warp * kTiles + i) * 32 + lane] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+        if ((lane & 3) == 0) {
+            ml[warp * 16 + r0] = ml0;
+            ml[warp * 16 + r0 + 8] = ml1;
+        }
+    }
+    cluster_barrier();
+    for (int t = warp * C + rank; t < MT * kTiles; t += kWarps * C) {
+        const int ht = t / kTiles, tile = t - ht * kTiles;
+        float2 a[kMaxCluster], b[kMaxCluster];
+        float4 v[kMaxCluster];
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r) {
+            a[r] = b[r] = make_float2(-INFINITY, 0.f);
+            v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < C) {
+                a[r] = ld_cluster2(peer(&ml[ht * 16 + r0], r));
+                b[r] = ld_cluster2(peer(&ml[ht * 16 + r0 + 8], r));
+                v[r] = ld_cluster4(peer(&box[t * 32 + lane], r));
+            }
+        }
+        float M0 = -INFINITY, M1 = -INFINITY, L0 = 0.f, L1 = 0.f;
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r) {
+            M0 = fmaxf(M0, a[r].x);
+            M1 = fmaxf(M1, b[r].x);
+        }
+        const float z0 = M0 == -INFINITY ? 0.f : M0, z1 = M1 == -INFINITY ? 0.f : M1;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r) {
+            const float f0 = ex2(a[r].x - z0), f1 = ex2(b[r].x - z1);
+            L0 += a[r].y * f0;
+            L1 += b[r].y * f1;
+            x.x += v[r].x * f0;
+            x.y += v[r].y * f0;
+            x.z += v[r].z * f1;
+            x.w += v[r].w * f1;
+        }
+        const float i0 = L0 != 0.f ? 1.f / L0 : 0.f, i1 = L1 != 0.f ? 1.f / L1 : 0.f;
+        const int left = p.G - ht * 16;
+        uint32_t *op = reinterpret_cast<uint32_t *>(
+            static_cast<uint8_t *>(p.out) + ((item * p.G + ht * 16 + r0) * D + tile * 8 + (lane & 3) * 2) * 2);
+        if (r0 < left) op[0] = Num<T>::pack(x.x * i0, x.y * i0);
+        if (r0 + 8 < left) op[4 * D] = Num<T>::pack(x.z * i1, x.w * i1);
+        if (p.lse && tile == 0 && (lane & 3) == 0) {
+            float *l = p.lse + item * p.G + ht * 16 + r0;
+            if (r0 < left) l[0] = L0 != 0.f ? (M0 + log2f(L0)) * kLn2 : -INFINITY;
+            if (r0 + 8 < left) l[8] = L1 != 0.f ? (M1 + log2f(L1)) * kLn2 : -INFINITY;
+        }
+    }
+    if (p.weights) {
+        if (tid < 16 * MT) {
+            float M = -INFINITY, L = 0.f;
+            float2 a[kMaxCluster];
+#pragma unroll
+            for (int r = 0; r < kMaxCluster; ++r) {
+                a[r] = r < C ? ld_cluster2(peer(&ml[tid], r)) : make_float2(-INFINITY, 0.f);
+                M = fmaxf(M, a[r].x);
+            }
+#pragma unroll
+            for (int r = 0; r < kMaxCluster; ++r) L += a[r].y * ex2(a[r].x - (M == -INFINITY ? 0.f : M));
+            z[tid] = L != 0.f ? M + log2f(L) : -INFINITY;
+        }
+    }
+    __syncwarp();
+    cluster_arrive();
+    if (p.weights) {
+        __syncthreads();
+        const int64_t b = item / p.Hk, g = item - b * p.Hk;
+        const int32_t end = min(u1 * kUnit, len);
+        for (int32_t pos = u0 * kUnit + 4 * tid; pos < end; pos += 4 * kThreads)
+            gather4(p, item, z, p.weights + b * p.w_sb + g * p.w_sh, pos, end);
+    }
+    cluster_wait();  // no block leaves while another reads its shared memory
+}
 
 template <int MT> __device__ __forceinline__ void team_sync(int team) {
     if (MT == 1) __syncwarp();
@@ -201,7 +365,8 @@ template <int D, int MT> struct Shape {
     static constexpr uint32_t kSmem = kTeams * kSlots * kSlot + kMerge;
 };
 
-template <typename T, int D, int MT>
+// kNear: a cluster has one item and joins it itself.
+template <typename T, int D, int MT, bool kNear>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __grid_constant__ Params p) {
     using S = Shape<D, MT>;
     constexpr int kTeams = S::kTeams, kStep = S::kStep, kSlots = S::kSlots, kRow = S::kRow;
@@ -217,6 +382,23 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
     const uint32_t ring = smem_u32(smem) + team * (kSlots * kSlot);
     float4 *merge = reinterpret_cast<float4 *>(smem + kTeams * kSlots * kSlot);  // [2][D / 8][32]
 
+    const int32_t C = kNear ? cluster_size() : 1, rank = kNear ? cluster_rank() : 0, me = blockIdx.x;
+    int32_t u0, u1;
+    Place in;  // where the loads are
+    Shares shares;
+    if constexpr (kNear) {
+        const int32_t item = me / C;
+        in.b = item / p.Hk;
+        in.h = item - in.b * p.Hk;
+        in.set(p, in.b);
+        if (in.len == 0) {
+            if (rank == 0) write_empty<D>(p, item, kThreads);
+            return;
+        }
+        shares = Shares(in.units, C);
+        u0 = in.unit = shares.begin(rank);
+        u1 = shares.begin(rank + 1);
+    } else {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // this block's share of the units
     const int32_t per = (p.B + kThreads - 1) / kThreads;
@@ -224,10 +406,11 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
     int32_t total, before = scan_units<kWarps>(p, b0, b1, warp_sums, total);
     before *= p.Hk;
     total *= p.Hk;
-    const int32_t workers = min((total + kGrain - 1) / kGrain, p.workers), me = blockIdx.x;
+    const int32_t workers = min((total + kGrain - 1) / kGrain, p.workers);
     if (me >= workers) return;
-    const Shares shares(total, workers);
-    const int32_t u0 = shares.begin(me), u1 = shares.begin(me + 1);
+    shares = Shares(total, workers);
+    u0 = shares.begin(me);
+    u1 = shares.begin(me + 1);
     for (int32_t b = b0; b < b1; ++b) {
         const int32_t n = units_of(length(p, b)), mine = n * p.Hk;
         if (u0 >= before && u0 < before + mine) {
@@ -239,10 +422,10 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
         before += mine;
     }
     __syncthreads();
-    Place in;  // where the loads are
     in.set(p, start[0]);
     in.h = start[1];
     in.unit = start[2];
+    }
     Place at = in;  // where the arithmetic is
     int32_t to_fetch = (u1 - u0) * S::kSteps;
     int in_k = 0;
@@ -306,9 +489,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
     const uint32_t k_at = k_row * kRow + ((((lane >> 3) & 1) ^ (k_row & 7)) << 4);
     const uint32_t v_at = v_row * kRow + (((lane >> 4) ^ (v_row & 7)) << 4);
     int32_t u = u0;
-    while (u < u1) {
+    while (kNear || u < u1) {  // kNear: once, also without a unit
         // one item's units in this block
-        const int32_t seg_end = min(u + (at.units - at.unit), u1);
+        const int32_t seg_end = kNear ? u1 : min(u + (at.units - at.unit), u1);
         const bool from_start = at.unit == 0, to_end = u + (at.units - at.unit) == seg_end;
         const int64_t item = (int64_t)at.b * p.Hk + at.h;
         const int32_t item_u0 = u - at.unit;
@@ -472,6 +655,10 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
             }
             __syncthreads();
         }
+        if constexpr (kNear) {
+            join_cluster<T, D, MT>(p, o, make_float2(m0, l0), make_float2(m1, l1), item, C, rank, u0, u1, at.len, smem);
+            return;
+        }
         if (team == 0) {
             if (from_start && to_end) {  // the whole item
                 const float i0 = l0 != 0.f ? 1.f / l0 : 0.f, i1 = l1 != 0.f ? 1.f / l1 : 0.f;
@@ -520,9 +707,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
 // 16-head tile, and slices = 16 / tiles warps share a tile's parts), and gathers weights (the other blocks y).  Blocks
 // x: items.  All of it is latency: every load of a thread that another does not need first is under way at once.
 template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p, int32_t tiles, int32_t splits) {
-    constexpr int kJoinWarps = kJoinThreads / 32, kMl = kMaxWorkers / 32, kBatch = 10;
-    __shared__ float factor[kMaxWorkers][16];  // of each part and head: 2^(m - M) / L
+__global__ void __launch_bounds__(kJoinThreads, 2) join_kernel(const __grid_constant__ Params p, int32_t tiles, int32_t splits) {
+    constexpr int kJoinWarps = kJoinThreads / 32, kBatch = 5;
+    __shared__ float2 ml[kMaxWorkers][17];  // of each part and head: maximum and sum.  17: banks
     __shared__ float4 sums[kJoinWarps][32];
     __shared__ __align__(16) float z[kMaxG];
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -532,46 +719,36 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     const bool join = (int)blockIdx.y < splits;
     const int2 sp = __ldcg(&p.span[item]);
     if (len == 0) {
-        if (blockIdx.y == 0) {
-            uint32_t *op = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p.out) + (int64_t)item * p.G * D * 2);
-            for (int i = tid; i < p.G * D / 2; i += kJoinThreads) op[i] = 0u;
-            if (p.lse)
-                for (int i = tid; i < p.G; i += kJoinThreads) p.lse[(int64_t)item * p.G + i] = -INFINITY;
-        }
+        if (blockIdx.y == 0) write_empty<D>(p, item, kJoinThreads);
         return;
     }
     const int32_t parts = sp.y - sp.x + 1;
     if (join && parts == 1) return;
     auto spot = [&](int32_t i) { return 2 * (int64_t)(sp.x + i) + (i == 0 ? 1 : 0); };
-    // M and L of each head of a tile: one warp a head
-    auto stats = [&](int ht, bool factors) {
-        float2 v[kMl];
-#pragma unroll
-        for (int j = 0; j < kMl; ++j) {
-            const int32_t i = lane + 32 * j;
-            v[j] = make_float2(-INFINITY, 0.f);
-            if (32 * j < parts && i < parts) v[j] = __ldcg(&p.part_ml[spot(i) * (16 * MT) + ht * 16 + warp]);
-        }
+    // M and L of each head of a tile, one warp a head; ml becomes 2^(m - M) / L of each part and head
+    auto stats = [&](int ht) {
+        for (int32_t i = tid; i < parts * 16; i += kJoinThreads)
+            ml[i >> 4][i & 15] = __ldcg(&p.part_ml[spot(i >> 4) * (16 * MT) + ht * 16 + (i & 15)]);
+        __syncthreads();
         float M = -INFINITY, L = 0.f;
-#pragma unroll
-        for (int j = 0; j < kMl; ++j) M = fmaxf(M, v[j].x);
+        for (int32_t i = lane; i < parts; i += 32) M = fmaxf(M, ml[i][warp].x);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
         const float base = M == -INFINITY ? 0.f : M;
-#pragma unroll
-        for (int j = 0; j < kMl; ++j) {
-            v[j].x = ex2(v[j].x - base);
-            L += v[j].y * v[j].x;
+        for (int32_t i = lane; i < parts; i += 32) {
+            const float2 v = ml[i][warp];
+            const float f = ex2(v.x - base);
+            L += v.y * f;
+            ml[i][warp].x = f;
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-        if (factors) {
-            const float inv = L != 0.f ? 1.f / L : 0.f;
-#pragma unroll
-            for (int j = 0; j < kMl; ++j)
-                if (lane + 32 * j < parts) factor[lane + 32 * j][warp] = v[j].x * inv;
-        }
-        return L != 0.f ? M + log2f(L) : -INFINITY;
+        const float inv = L != 0.f ? 1.f / L : 0.f;
+        for (int32_t i = lane; i < parts; i += 32) ml[i][warp].x *= inv;
+        const float lse2 = L != 0.f ? M + log2f(L) : -INFINITY;
+        if (lane == 0) z[ht * 16 + warp] = lse2;
+        __syncthreads();
+        return lse2;
     };
     if (join) {
         const int slices = kJoinWarps / tiles, per_ht = D / 8 / tiles;
@@ -585,10 +762,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
                 if (i + j * slices < parts) v[j] = __ldcg(src + spot(i + j * slices) * (MT * (D / 8) * 32));
         };
         load(i0);  // while M and L are found
-        const float lse2 = stats(ht, true);
+        const float lse2 = stats(ht);
         if (p.lse && blockIdx.y % per_ht == 0 && lane == 0 && ht * 16 + warp < p.G)
             p.lse[(int64_t)item * p.G + ht * 16 + warp] = lse2 * kLn2;
-        __syncthreads();
         const int r0 = lane >> 2;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int32_t i = i0; i < parts; i += kBatch * slices) {
@@ -596,7 +772,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 #pragma unroll
             for (int j = 0; j < kBatch; ++j)
                 if (i + j * slices < parts) {
-                    const float f0 = factor[i + j * slices][r0], f1 = factor[i + j * slices][r0 + 8];
+                    const float f0 = ml[i + j * slices][r0].x, f1 = ml[i + j * slices][r0 + 8].x;
                     acc.x += v[j].x * f0;
                     acc.y += v[j].y * f0;
                     acc.z += v[j].z * f1;
@@ -626,38 +802,12 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     if (parts == 1) {
         if (tid < p.G) z[tid] = __ldcg(&p.lse2[(int64_t)item * (16 * MT) + tid]);
     } else {
-        for (int ht = 0; ht < MT; ++ht) {
-            const float lse2 = stats(ht, false);
-            if (lane == 0) z[ht * 16 + warp] = lse2;
-        }
+        for (int ht = 0; ht < MT; ++ht) stats(ht);
     }
     __syncthreads();
-    const float *sc = p.scores + (int64_t)item * p.G * p.score_ld;
-    float *w = p.weights + b * p.w_sb + g * p.w_sh;
     const int32_t n_blocks = gridDim.y - splits, mine = blockIdx.y - splits;
-    for (int64_t pos = 4 * ((int64_t)mine * kJoinThreads + tid); pos < len; pos += 4 * (int64_t)n_blocks * kJoinThreads) {
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        // positions not held have a score of -inf: they gather nothing, even where the head's lse is NaN
-        auto term = [](float s, float zh) { return s == -INFINITY || zh == -INFINITY ? 0.f : ex2(s - zh); };
-        const int32_t n = min(4, (int32_t)(len - pos));
-        float old[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i < n) old[i] = w[pos + i];
-#pragma unroll 8
-        for (int h = 0; h < p.G; ++h) {
-            const float4 s = __ldcs(reinterpret_cast<const float4 *>(sc + h * p.score_ld + pos));
-            const float zh = z[h];
-            x.x += term(s.x, zh);
-            x.y += term(s.y, zh);
-            x.z += term(s.z, zh);
-            x.w += term(s.w, zh);
-        }
-        const float add[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i < n) w[pos + i] = old[i] + add[i];
-    }
+    for (int64_t pos = 4 * ((int64_t)mine * kJoinThreads + tid); pos < len; pos += 4 * (int64_t)n_blocks * kJoinThreads)
+        gather4(p, item, z, p.weights + b * p.w_sb + g * p.w_sh, (int32_t)pos, len);
 }
 
 int64_t workers_of_device() {
@@ -692,12 +842,40 @@ Layout layout_of(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t max_len, 
     return l;
 }
 
+// Blocks of a cluster that has one item, or 0 where the work is dealt out evenly instead.  A cluster joins its item itself,
+// without a second kernel, but its blocks idle where other sequences are longer: it pays where every item at its longest
+// is short work for its blocks and all are resident at once.
+int cluster_for(const Params &p, int64_t D) {
+    const int64_t units = ((int64_t)p.max_len + kUnit - 1) / kUnit, items = (int64_t)p.B * p.Hk;
+    int64_t C = 1;
+    while (C < kMaxCluster && C < units && items * C * 2 <= workers_of_device()) C *= 2;
+    return items * C <= workers_of_device() && (units + C - 1) / C * D <= kNearUnits * 128 ? (int)C : 0;
+}
+
 template <typename T, int D, int MT> int launch(const Params &p, cudaStream_t s) {
     constexpr uint32_t smem = Shape<D, MT>::kSmem;
-    UNUM_CHECK_CUDA(cudaFuncSetAttribute(attend_kernel<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    attend_kernel<T, D, MT><<<(unsigned)p.workers, kThreads, smem, s>>>(p);
-    if (int rc = unum::check_launch("attend_kernel")) return rc;
     const int64_t items = (int64_t)p.B * p.Hk;
+    if (const int C = cluster_for(p, D)) {
+        auto *kernel = attend_kernel<T, D, MT, true>;
+        UNUM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(items * C));
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = s;
+        cudaLaunchAttribute attr = {};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = (unsigned)C;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        UNUM_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+        return unum::check_launch("attend_kernel");
+    }
+    auto *kernel = attend_kernel<T, D, MT, false>;
+    UNUM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    kernel<<<(unsigned)p.workers, kThreads, smem, s>>>(p);
+    if (int rc = unum::check_launch("attend_kernel")) return rc;
     // A long item is cut into about workers / items parts, and then a block of the second kernel has one tile's columns
     // and 16 warps on its parts; where items are many they have a few parts each, and a block has the whole row.
     int tiles = D / 8;
