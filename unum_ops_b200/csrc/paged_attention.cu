@@ -36,13 +36,13 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kBlocksPerSm = 2;
-constexpr int kUnit = 64;            // positions dealt to a block at a time
 constexpr int kGrain = 2;            // units a block takes at least: below it the join costs more than the split gains
 constexpr int kMaxWorkers = 296;     // resident blocks, at most: two on each of 148 SMs
 constexpr uint32_t kRingBytes = 96 * 1024;
 constexpr int kMaxG = 64;
+constexpr int kMaxUnit = 128;
 constexpr int kMaxCluster = 8;
-constexpr int kNearUnits = 8;        // of a cluster's block, at most (at head dim 128)
+constexpr int kNearWork = 512 * 128;  // positions times head dim of a cluster's block, at most
 constexpr int kJoinThreads = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -75,6 +75,9 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32
     asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(bytes),
                  "l"(policy)
                  : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ uint64_t evict_first() {
     uint64_t policy;
@@ -166,15 +169,14 @@ __device__ __forceinline__ int32_t length(const Params &p, int32_t b) {
     const int32_t n = __ldg(p.lens + b);
     return n < 0 ? 0 : (n > p.max_len ? p.max_len : n);
 }
-__device__ __forceinline__ int32_t units_of(int32_t len) { return (len + kUnit - 1) / kUnit; }
 
 // A place in the row of units: sequence, kv head, unit of the item.
-struct Place {
+template <int kUnit> struct Place {
     int32_t b, h, unit, units, len;
     __device__ __forceinline__ void set(const Params &p, int32_t b_) {
         b = b_;
         len = b < p.B ? length(p, b) : 0;
-        units = units_of(len);
+        units = (len + kUnit - 1) / kUnit;
     }
     __device__ __forceinline__ void next_item(const Params &p) {
         unit = 0;
@@ -189,11 +191,11 @@ struct Place {
 };
 
 // Units before this thread's share of the sequences, and the total (over one kv head).  All threads call it.
-template <int kN>
+template <int kN, int kUnit>
 __device__ __forceinline__ int32_t scan_units(const Params &p, int32_t b0, int32_t b1, int32_t *warp_sums, int32_t &total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int32_t mine = 0;
-    for (int32_t b = b0; b < b1; ++b) mine += units_of(length(p, b));
+    for (int32_t b = b0; b < b1; ++b) mine += (length(p, b) + kUnit - 1) / kUnit;
     int32_t x = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -222,6 +224,22 @@ struct Shares {
         const int32_t edge = more * (base + 1);
         return u < edge ? u / (base + 1) : more + (u - edge) / base;
     }
+};
+
+// MT = 16-head tiles of a group (1, 2 or 4): the warps of a team.  A team's step is 16 positions, or 32 where the ring has
+// room for three such: the steps' barriers, maxima and copies cost half as much a position.  A unit, what is dealt out at
+// a time, has a step for every team at least.
+template <int D, int MT> struct Shape {
+    static constexpr int kTeams = kWarps / MT, kStep = MT == 1 && D == 128 ? 16 : 32, kRow = D * 2;  // kRow in bytes
+    static constexpr int kUnit = kTeams * kStep > 64 ? kTeams * kStep : 64;
+    static constexpr int kSteps = kUnit / (kTeams * kStep);             // a team's steps in a unit
+    static constexpr uint32_t kHalf = kStep * kRow, kSlot = 2 * kHalf;  // keys, values of a step
+    static constexpr int kFit = kRingBytes / (kTeams * kSlot), kSlots = kFit > 8 ? 8 : kFit;
+    // shared memory: the ring, what the teams leave for the first one (half of their columns at a time), the entries of
+    // the table that each warp has read ahead
+    static constexpr int kBox = (D / 16) * 32 * 16;
+    static constexpr uint32_t kMergeAt = kTeams * kSlots * kSlot, kEntriesAt = kMergeAt + (kTeams - 1) * MT * kBox;
+    static constexpr uint32_t kSmem = kEntriesAt + kWarps * kSlots * kStep * 4;
 };
 
 template <int D> __device__ __forceinline__ void write_empty(const Params &p, int64_t item, int threads) {
@@ -279,6 +297,7 @@ __device__ __forceinline__ void join_cluster(const Params &p, const float (&o)[D
         }
     }
     cluster_barrier();
+    constexpr int kUnit = Shape<D, MT>::kUnit;
     for (int t = warp * C + rank; t < MT * kTiles; t += kWarps * C) {
         const int ht = t / kTiles, tile = t - ht * kTiles;
         float2 a[kMaxCluster], b[kMaxCluster];
@@ -354,37 +373,28 @@ template <int MT> __device__ __forceinline__ void team_sync(int team) {
     else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(MT * 32) : "memory");
 }
 
-// MT = 16-head tiles of a group (1, 2 or 4): the warps of a team.  A team's step is 16 positions, or 32 where a team has
-// several warps and so more room in the ring: the steps' barriers, maxima and copies cost half as much a position.
-template <int D, int MT> struct Shape {
-    static constexpr int kTeams = kWarps / MT, kStep = MT == 1 ? 16 : 32, kRow = D * 2;  // kRow in bytes
-    static constexpr int kSteps = kUnit / (kTeams * kStep);                               // a team's steps in a unit
-    static constexpr uint32_t kHalf = kStep * kRow, kSlot = 2 * kHalf;                    // keys, values of a step
-    static constexpr int kFit = kRingBytes / (kTeams * kSlot), kSlots = kFit > 8 ? 8 : kFit;
-    static constexpr uint32_t kMerge = kTeams > 1 ? 2 * (D / 8) * 32 * 16 : 0;
-    static constexpr uint32_t kSmem = kTeams * kSlots * kSlot + kMerge;
-};
-
 // kNear: a cluster has one item and joins it itself.
 template <typename T, int D, int MT, bool kNear>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __grid_constant__ Params p) {
     using S = Shape<D, MT>;
-    constexpr int kTeams = S::kTeams, kStep = S::kStep, kSlots = S::kSlots, kRow = S::kRow;
+    constexpr int kTeams = S::kTeams, kStep = S::kStep, kSlots = S::kSlots, kRow = S::kRow, kUnit = S::kUnit;
     constexpr uint32_t kHalf = S::kHalf, kSlot = S::kSlot;
     constexpr int kLanes = kRow / 16, kRows = 32 / kLanes;  // lanes of a row, rows of one copy instruction
     constexpr int kCopies = kStep / kRows / MT;             // of each warp, for keys and for values
     static_assert(kCopies >= 1 && kSlots >= 3, "a step must give every warp a copy");
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ uint32_t held[kTeams][8];                 // which of a slot's positions are valid
+    __shared__ uint32_t held[kTeams][kSlots];            // which of a slot's positions are held
+    __shared__ int2 ahead[kWarps][kSlots];               // of a step whose entries are read ahead: kv head, first position
     __shared__ int32_t warp_sums[kWarps], start[3];
-    __shared__ float2 merge_ml[2][16];
+    __shared__ float2 merge_ml[(kTeams > 1 ? kTeams - 1 : 1) * MT][16];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, team = warp / MT, ht = warp % MT;
     const uint32_t ring = smem_u32(smem) + team * (kSlots * kSlot);
-    float4 *merge = reinterpret_cast<float4 *>(smem + kTeams * kSlots * kSlot);  // [2][D / 8][32]
+    float4 *merge = reinterpret_cast<float4 *>(smem + S::kMergeAt);
+    int32_t *entries = reinterpret_cast<int32_t *>(smem + S::kEntriesAt) + warp * (kSlots * kStep) + (lane & (kStep - 1));
 
     const int32_t C = kNear ? cluster_size() : 1, rank = kNear ? cluster_rank() : 0, me = blockIdx.x;
     int32_t u0, u1;
-    Place in;  // where the loads are
+    Place<kUnit> in;  // where the entries are read
     Shares shares;
     if constexpr (kNear) {
         const int32_t item = me / C;
@@ -403,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
     // this block's share of the units
     const int32_t per = (p.B + kThreads - 1) / kThreads;
     const int32_t b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
-    int32_t total, before = scan_units<kWarps>(p, b0, b1, warp_sums, total);
+    int32_t total, before = scan_units<kWarps, kUnit>(p, b0, b1, warp_sums, total);
     before *= p.Hk;
     total *= p.Hk;
     const int32_t workers = min((total + kGrain - 1) / kGrain, p.workers);
@@ -412,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
     u0 = shares.begin(me);
     u1 = shares.begin(me + 1);
     for (int32_t b = b0; b < b1; ++b) {
-        const int32_t n = units_of(length(p, b)), mine = n * p.Hk;
+        const int32_t n = (length(p, b) + kUnit - 1) / kUnit, mine = n * p.Hk;
         if (u0 >= before && u0 < before + mine) {
             const int32_t r = u0 - before;
             start[0] = b;
@@ -426,29 +436,29 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
     in.h = start[1];
     in.unit = start[2];
     }
-    Place at = in;  // where the arithmetic is
+    Place<kUnit> at = in;  // where the arithmetic is
     int32_t to_fetch = (u1 - u0) * S::kSteps;
     int in_k = 0;
 
-    // the next step's token of position lane % kStep (or -1), read ahead of its copies
-    int32_t tok = -1, tok_h = 0;
-    auto fetch = [&]() {
-        tok = -1;
-        if (to_fetch == 0) return;
-        const int32_t pos = in.unit * kUnit + (team + kTeams * in_k) * kStep + (lane & (kStep - 1));
-        tok_h = in.h;
-        if (pos < in.len) {
-            const int64_t page = __ldg(p.table + in.b * p.bt_stride + (pos >> p.shift));
-            const int64_t t = (page << p.shift) + (pos & ((1 << p.shift) - 1));
-            tok = page >= 0 && t < p.n_tokens ? (int32_t)t : -1;
+    // Reads a step's table entries, lane % kStep for a position, on their way to shared memory: they are wanted
+    // kSlots - 1 steps before the step's own turn, and come with the copies of the step that is waited for then.
+    auto read_ahead = [&](uint32_t slot) {
+        int32_t *to = entries + slot * kStep;
+        if (to_fetch == 0) {
+            *to = -1;
+            return;
         }
+        const int32_t pos0 = in.unit * kUnit + (team + kTeams * in_k) * kStep, pos = pos0 + (lane & (kStep - 1));
+        if (pos >= in.len) *to = -1;
+        else if (lane < kStep) cp_async4(smem_u32(to), p.table + in.b * p.bt_stride + (pos >> p.shift));
+        if (lane == 0) ahead[warp][slot] = make_int2(in.h, pos0);
         --to_fetch;
         if (++in_k == S::kSteps) {
             in_k = 0;
             in.next(p);
         }
     };
-    // its copies into a slot.  Rows of positions that are not held are zeroed: what their memory holds would reach
+    // A step's copies into its slot.  Rows of positions that are not held are zeroed: what their memory holds would reach
     // the output as 0 * NaN.  (Copies without that check where all 16 are held: the branch cost 8%.)
     constexpr uint32_t kAll = kStep == 32 ? 0xffffffffu : 0xffffu;
     const int copy_row = ht * kRows + lane / kLanes;
@@ -458,11 +468,15 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
     // 55.3 -> 51.4 us; 131072 positions 39.3 -> 38.0 us).
     const uint64_t policy = evict_first();
     auto issue = [&](uint32_t slot) {
+        const int2 step = ahead[warp][slot];
+        const int64_t page = entries[slot * kStep];
+        const int64_t token = (page << p.shift) + ((step.y + (lane & (kStep - 1))) & ((1 << p.shift) - 1));
+        const int32_t tok = page >= 0 && token < p.n_tokens ? (int32_t)token : -1;
         const uint32_t mask = __ballot_sync(0xffffffffu, tok >= 0) & kAll;
         if (ht == 0 && lane == 0) held[team][slot] = mask;
         if (mask) {
-            const uint8_t *kb = p.kc + tok_h * p.k_sh + copy_chunk * 16;
-            const uint8_t *vb = p.vc + tok_h * p.v_sh + copy_chunk * 16;
+            const uint8_t *kb = p.kc + step.x * p.k_sh + copy_chunk * 16;
+            const uint8_t *vb = p.vc + step.x * p.v_sh + copy_chunk * 16;
             const uint32_t to = copy_to + slot * kSlot;
 #pragma unroll
             for (int i = 0; i < kCopies; ++i) {
@@ -474,11 +488,15 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
                 cp_async16(dst + kHalf, vb + o * p.v_st, t < 0 ? 0u : 16u, policy);
             }
         }
+        read_ahead(slot == 0 ? kSlots - 1 : slot - 1);
         cp_commit();
-        fetch();
     };
 
-    fetch();
+#pragma unroll 1
+    for (int s = 0; s < kSlots - 1; ++s) read_ahead(s);
+    cp_commit();
+    cp_wait<0>();
+    __syncwarp();
 #pragma unroll 1
     for (int s = 0; s < kSlots - 1; ++s) issue(s);
 
@@ -621,39 +639,67 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
             l0 += __shfl_xor_sync(0xffffffffu, l0, i);
             l1 += __shfl_xor_sync(0xffffffffu, l1, i);
         }
-        // the teams' parts, halving: the upper half leaves its own, the lower half takes it in
-#pragma unroll
-        for (int half = kTeams / 2; half >= 1; half >>= 1) {
-            const int spot = (team % half) * MT + ht;  // at most two
-            float4 *box = merge + spot * (D / 8) * 32 + lane;
-            if (team >= half && team < 2 * half) {
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) box[i * 32] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
-                if ((lane & 3) == 0) {
-                    merge_ml[spot][r0] = make_float2(m0, l0);
-                    merge_ml[spot][r0 + 8] = make_float2(m1, l1);
-                }
+        // the first team takes in what the others leave, half of the columns at a time
+        if constexpr (kTeams > 1) {
+            if (team > 0 && (lane & 3) == 0) {
+                merge_ml[warp - MT][r0] = make_float2(m0, l0);
+                merge_ml[warp - MT][r0 + 8] = make_float2(m1, l1);
             }
-            __syncthreads();
-            if (team < half) {
-                const float2 y0 = merge_ml[spot][r0], y1 = merge_ml[spot][r0 + 8];
-                const float n0 = fmaxf(m0, y0.x), n1 = fmaxf(m1, y1.x);
-                const float z0 = n0 == -INFINITY ? 0.f : n0, z1 = n1 == -INFINITY ? 0.f : n1;
-                const float a0 = ex2(m0 - z0), a1 = ex2(m1 - z1), e0 = ex2(y0.x - z0), e1 = ex2(y1.x - z1);
-                m0 = n0;
-                m1 = n1;
-                l0 = l0 * a0 + y0.y * e0;
-                l1 = l1 * a1 + y1.y * e1;
+            float f0[kTeams], f1[kTeams];
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    const float4 y = box[i * 32];
-                    o[i][0] = o[i][0] * a0 + y.x * e0;
-                    o[i][1] = o[i][1] * a0 + y.y * e0;
-                    o[i][2] = o[i][2] * a1 + y.z * e1;
-                    o[i][3] = o[i][3] * a1 + y.w * e1;
+            for (int half = 0; half < 2; ++half) {
+                if (team > 0) {
+                    float4 *box = merge + (warp - MT) * (D / 16) * 32 + lane;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        const float(&x)[4] = o[half * (D / 16) + i];
+                        box[i * 32] = make_float4(x[0], x[1], x[2], x[3]);
+                    }
                 }
+                __syncthreads();
+                if (team == 0) {
+                    if (half == 0) {
+                        float n0 = m0, n1 = m1;
+#pragma unroll
+                        for (int w = 1; w < kTeams; ++w) {
+                            n0 = fmaxf(n0, merge_ml[(w - 1) * MT + ht][r0].x);
+                            n1 = fmaxf(n1, merge_ml[(w - 1) * MT + ht][r0 + 8].x);
+                        }
+                        const float z0 = n0 == -INFINITY ? 0.f : n0, z1 = n1 == -INFINITY ? 0.f : n1;
+                        f0[0] = ex2(m0 - z0);
+                        f1[0] = ex2(m1 - z1);
+                        m0 = n0;
+                        m1 = n1;
+                        l0 *= f0[0];
+                        l1 *= f1[0];
+#pragma unroll
+                        for (int w = 1; w < kTeams; ++w) {
+                            const float2 y0 = merge_ml[(w - 1) * MT + ht][r0], y1 = merge_ml[(w - 1) * MT + ht][r0 + 8];
+                            f0[w] = ex2(y0.x - z0);
+                            f1[w] = ex2(y1.x - z1);
+                            l0 += y0.y * f0[w];
+                            l1 += y1.y * f1[w];
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        float(&x)[4] = o[half * (D / 16) + i];
+                        x[0] *= f0[0];
+                        x[1] *= f0[0];
+                        x[2] *= f1[0];
+                        x[3] *= f1[0];
+#pragma unroll
+                        for (int w = 1; w < kTeams; ++w) {
+                            const float4 y = merge[(((w - 1) * MT + ht) * (D / 16) + i) * 32 + lane];
+                            x[0] += y.x * f0[w];
+                            x[1] += y.y * f0[w];
+                            x[2] += y.z * f1[w];
+                            x[3] += y.w * f1[w];
+                        }
+                    }
+                }
+                __syncthreads();
             }
-            __syncthreads();
         }
         if constexpr (kNear) {
             join_cluster<T, D, MT>(p, o, make_float2(m0, l0), make_float2(m1, l1), item, C, rank, u0, u1, at.len, smem);
@@ -836,7 +882,7 @@ Layout layout_of(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t max_len, 
     l.part_ml = take(2 * W * rows * 8);
     l.span = take(items * 8);
     l.lse2 = take(items * rows * 4);
-    l.score_ld = (max_len + kUnit - 1) / kUnit * kUnit;
+    l.score_ld = (max_len + kMaxUnit - 1) / kMaxUnit * kMaxUnit;
     l.scores = take(gather ? items * (Hq / Hk) * l.score_ld * 4 : 0);
     l.bytes = at;
     return l;
@@ -845,17 +891,17 @@ Layout layout_of(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t max_len, 
 // Blocks of a cluster that has one item, or 0 where the work is dealt out evenly instead.  A cluster joins its item itself,
 // without a second kernel, but its blocks idle where other sequences are longer: it pays where every item at its longest
 // is short work for its blocks and all are resident at once.
-int cluster_for(const Params &p, int64_t D) {
-    const int64_t units = ((int64_t)p.max_len + kUnit - 1) / kUnit, items = (int64_t)p.B * p.Hk;
+int cluster_for(const Params &p, int64_t D, int64_t unit) {
+    const int64_t units = ((int64_t)p.max_len + unit - 1) / unit, items = (int64_t)p.B * p.Hk;
     int64_t C = 1;
     while (C < kMaxCluster && C < units && items * C * 2 <= workers_of_device()) C *= 2;
-    return items * C <= workers_of_device() && (units + C - 1) / C * D <= kNearUnits * 128 ? (int)C : 0;
+    return items * C <= workers_of_device() && (units + C - 1) / C * unit * D <= kNearWork ? (int)C : 0;
 }
 
 template <typename T, int D, int MT> int launch(const Params &p, cudaStream_t s) {
     constexpr uint32_t smem = Shape<D, MT>::kSmem;
     const int64_t items = (int64_t)p.B * p.Hk;
-    if (const int C = cluster_for(p, D)) {
+    if (const int C = cluster_for(p, D, Shape<D, MT>::kUnit)) {
         auto *kernel = attend_kernel<T, D, MT, true>;
         UNUM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         cudaLaunchConfig_t cfg = {};
@@ -945,9 +991,9 @@ extern "C" int unum_paged_attention(const void *q, int64_t B, int64_t Hq, int64_
     UNUM_CHECK_ARG(k_st >= 0 && k_st < (1 << 30) && v_st >= 0 && v_st < (1 << 30),
                    "token strides of k_cache and v_cache must be below 2^30 elements");
     UNUM_CHECK_ARG(Hk < 65536 && B < ((int64_t)1 << 31) / Hk &&
-                       B * Hk < ((int64_t)1 << 31) / ((max_seqlen + kUnit - 1) / kUnit + 1),
+                       B * Hk < ((int64_t)1 << 31) / (max_seqlen / 64 + 2),
                    "too many sequences, kv heads or positions");
-    UNUM_CHECK_ARG(max_seqlen <= ((int64_t)1 << 31) - 2 * kUnit && n_tokens < ((int64_t)1 << 31),
+    UNUM_CHECK_ARG(max_seqlen <= ((int64_t)1 << 31) - 2 * kMaxUnit && n_tokens < ((int64_t)1 << 31),
                    "max_seqlen and n_tokens must stay below 2^31");
     const Layout l = layout_of(B, Hq, Hk, D, max_seqlen, weights != nullptr);
     if (workspace_bytes < l.bytes || !workspace || !unum::aligned16(workspace)) {
@@ -970,7 +1016,7 @@ extern "C" int unum_paged_attention(const void *q, int64_t B, int64_t Hq, int64_
     p.Hk = (int32_t)Hk;
     p.G = (int32_t)(Hq / Hk);
     // no more blocks than the lengths can give units to
-    const int64_t most = B * Hk * ((max_seqlen + kUnit - 1) / kUnit), W = workers_of_device();
+    const int64_t most = B * Hk * ((max_seqlen + 63) / 64), W = workers_of_device();
     p.workers = (int32_t)(most < 1 ? 1 : (most < W ? most : W));
     p.c = softmax_scale * kLog2e;
     p.out = out;
