@@ -29,21 +29,24 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
 constexpr int kBlocksPerSm = 2;
 constexpr int kGrain = 2;            // units a block takes at least: below it the join costs more than the split gains
 constexpr int kMaxWorkers = 296;     // resident blocks, at most: two on each of 148 SMs
-constexpr uint32_t kRingBytes = 96 * 1024;
+constexpr uint32_t kRingBytes = 96 * 1024;      // two blocks an SM
+constexpr uint32_t kNearRingBytes = 192 * 1024;  // one: clusters that join their items have SMs to themselves
 constexpr int kMaxG = 64;
-constexpr int kMaxUnit = 128;
-constexpr int kMaxCluster = 8;
-constexpr int kNearWork = 512 * 128;  // positions times head dim of a cluster's block, at most
+constexpr int kMaxDevices = 64;
+constexpr int kMaxUnit = 256;
+constexpr int kMaxCluster = 16;
+constexpr int kNearWork = 1024 * 128;  // positions times head dim of a cluster's block, at most
 constexpr int kJoinThreads = 512;
+constexpr float kLag = 6.f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -229,17 +232,19 @@ struct Shares {
 // MT = 16-head tiles of a group (1, 2 or 4): the warps of a team.  A team's step is 16 positions, or 32 where the ring has
 // room for three such: the steps' barriers, maxima and copies cost half as much a position.  A unit, what is dealt out at
 // a time, has a step for every team at least.
-template <int D, int MT> struct Shape {
-    static constexpr int kTeams = kWarps / MT, kStep = MT == 1 && D == 128 ? 16 : 32, kRow = D * 2;  // kRow in bytes
+template <int D, int MT, bool kNear> struct Shape {
+    static constexpr int kWarps = kNear ? 8 : 4, kThreads = kWarps * 32, kTeams = kWarps / MT;
+    static constexpr int kStep = MT == 1 && D == 128 ? 16 : 32, kRow = D * 2;  // kRow in bytes
     static constexpr int kUnit = kTeams * kStep > 64 ? kTeams * kStep : 64;
     static constexpr int kSteps = kUnit / (kTeams * kStep);             // a team's steps in a unit
     static constexpr uint32_t kHalf = kStep * kRow, kSlot = 2 * kHalf;  // keys, values of a step
-    static constexpr int kFit = kRingBytes / (kTeams * kSlot), kSlots = kFit > 8 ? 8 : kFit;
-    // shared memory: the ring, what the teams leave for the first one (half of their columns at a time), the entries of
-    // the table that each warp has read ahead
-    static constexpr int kBox = (D / 16) * 32 * 16;
+    static constexpr int kFit = (kNear ? kNearRingBytes : kRingBytes) / (kTeams * kSlot), kSlots = kFit > 8 ? 8 : kFit;
+    // shared memory: the ring, what the teams leave for the first one (half of their columns at a time; a cluster's block
+    // has the ring for that), the entries of the table that each warp has read ahead
+    static constexpr int kBox = kNear ? 0 : (D / 16) * 32 * 16;
     static constexpr uint32_t kMergeAt = kTeams * kSlots * kSlot, kEntriesAt = kMergeAt + (kTeams - 1) * MT * kBox;
     static constexpr uint32_t kSmem = kEntriesAt + kWarps * kSlots * kStep * 4;
+    static_assert(!kNear || kMergeAt >= (kWarps + MT) * (D / 8) * 32 * 16, "a cluster's block joins in the ring");
 };
 
 template <int D> __device__ __forceinline__ void write_empty(const Params &p, int64_t item, int threads) {
@@ -274,87 +279,111 @@ __device__ __forceinline__ void gather4(const Params &p, int64_t item, const flo
         if (pos + i < end) w[pos + i] = old[i] + add[i];
 }
 
-// The end of an item that a cluster has: each block's first team leaves its output, maxima and sums (ml: of rows r0 and
-// r0 + 8) in shared memory, each block joins some of the 8-column tiles, in the order of the positions, and gathers the
-// weights of its own positions.
+// What parts of one tile (rows r0 and r0 + 8 of a lane) add up to: maxima in base 2, sums, outputs.
+struct Joined {
+    float2 ml0, ml1;
+    float4 o;
+    __device__ __forceinline__ Joined()
+        : ml0(make_float2(-INFINITY, 0.f)), ml1(make_float2(-INFINITY, 0.f)), o(make_float4(0.f, 0.f, 0.f, 0.f)) {}
+    // Takes in n parts, four under way at once.  A loop and not unrolled: code that runs once waits for its instructions.
+    template <typename Load> __device__ __forceinline__ void add(int n, const Load &load) {
+#pragma unroll 1
+        for (int i = 0; i < n; i += 4) {
+            float2 a[4], b[4];
+            float4 v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                a[e] = b[e] = make_float2(-INFINITY, 0.f);
+                v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i + e < n) load(i + e, a[e], b[e], v[e]);
+            }
+            const float M0 = fmaxf(fmaxf(ml0.x, fmaxf(a[0].x, a[1].x)), fmaxf(a[2].x, a[3].x));
+            const float M1 = fmaxf(fmaxf(ml1.x, fmaxf(b[0].x, b[1].x)), fmaxf(b[2].x, b[3].x));
+            const float z0 = M0 == -INFINITY ? 0.f : M0, z1 = M1 == -INFINITY ? 0.f : M1;
+            float f0 = ex2(ml0.x - z0), f1 = ex2(ml1.x - z1);
+            ml0 = make_float2(M0, ml0.y * f0);
+            ml1 = make_float2(M1, ml1.y * f1);
+            o = make_float4(o.x * f0, o.y * f0, o.z * f1, o.w * f1);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                f0 = ex2(a[e].x - z0);
+                f1 = ex2(b[e].x - z1);
+                ml0.y += a[e].y * f0;
+                ml1.y += b[e].y * f1;
+                o.x += v[e].x * f0;
+                o.y += v[e].y * f0;
+                o.z += v[e].z * f1;
+                o.w += v[e].w * f1;
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ float lse2_of(float2 ml) { return ml.y != 0.f ? ml.x + log2f(ml.y) : -INFINITY; }
+
+// The end of an item that a cluster has: the block's warps leave their outputs, maxima and sums (ml: of rows r0 and
+// r0 + 8) in shared memory and join them, tile by tile (8 columns of 16 heads); then each block joins some tiles of all
+// blocks, and gathers the weights of its own positions.  All in the order of the warps and blocks: the same bits each time.
 template <typename T, int D, int MT>
 __device__ __forceinline__ void join_cluster(const Params &p, const float (&o)[D / 8][4], float2 ml0, float2 ml1, int64_t item,
                                              int32_t C, int32_t rank, int32_t u0, int32_t u1, int32_t len, uint8_t *smem) {
-    __shared__ float2 ml[16 * MT];
+    using S = Shape<D, MT, true>;
+    constexpr int kTiles = D / 8, kWarps = S::kWarps, kThreads = S::kThreads, kUnit = S::kUnit, kTeams = S::kTeams;
+    __shared__ float2 warp_ml[kWarps][16], ml[16 * MT];
     __shared__ float z[16 * MT];
-    constexpr int kTiles = D / 8;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r0 = lane >> 2;
-    float4 *box = reinterpret_cast<float4 *>(smem);  // [MT][kTiles][32], where the ring was
+    float4 *boxes = reinterpret_cast<float4 *>(smem);  // [kWarps][kTiles][32], where the ring was
+    float4 *box = boxes + kWarps * kTiles * 32;        // [MT][kTiles][32]
     cp_wait<0>();
     __syncthreads();
-    if (warp < MT) {  // the first team
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i)
-            box[(warp * kTiles + i) * 32 + lane] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
-        if ((lane & 3) == 0) {
-            ml[warp * 16 + r0] = ml0;
-            ml[warp * 16 + r0 + 8] = ml1;
+    for (int i = 0; i < kTiles; ++i) boxes[(warp * kTiles + i) * 32 + lane] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+    if ((lane & 3) == 0) {
+        warp_ml[warp][r0] = ml0;
+        warp_ml[warp][r0 + 8] = ml1;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int t = warp; t < MT * kTiles; t += kWarps) {
+        const int ht = t / kTiles, tile = t - ht * kTiles;
+        Joined j;
+        j.add(kTeams, [&](int w, float2 &a, float2 &b, float4 &v) {
+            a = warp_ml[w * MT + ht][r0];
+            b = warp_ml[w * MT + ht][r0 + 8];
+            v = boxes[((w * MT + ht) * kTiles + tile) * 32 + lane];
+        });
+        box[t * 32 + lane] = j.o;
+        if (tile == 0 && (lane & 3) == 0) {
+            ml[ht * 16 + r0] = j.ml0;
+            ml[ht * 16 + r0 + 8] = j.ml1;
         }
     }
     cluster_barrier();
-    constexpr int kUnit = Shape<D, MT>::kUnit;
+#pragma unroll 1
     for (int t = warp * C + rank; t < MT * kTiles; t += kWarps * C) {
         const int ht = t / kTiles, tile = t - ht * kTiles;
-        float2 a[kMaxCluster], b[kMaxCluster];
-        float4 v[kMaxCluster];
-#pragma unroll
-        for (int r = 0; r < kMaxCluster; ++r) {
-            a[r] = b[r] = make_float2(-INFINITY, 0.f);
-            v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < C) {
-                a[r] = ld_cluster2(peer(&ml[ht * 16 + r0], r));
-                b[r] = ld_cluster2(peer(&ml[ht * 16 + r0 + 8], r));
-                v[r] = ld_cluster4(peer(&box[t * 32 + lane], r));
-            }
-        }
-        float M0 = -INFINITY, M1 = -INFINITY, L0 = 0.f, L1 = 0.f;
-#pragma unroll
-        for (int r = 0; r < kMaxCluster; ++r) {
-            M0 = fmaxf(M0, a[r].x);
-            M1 = fmaxf(M1, b[r].x);
-        }
-        const float z0 = M0 == -INFINITY ? 0.f : M0, z1 = M1 == -INFINITY ? 0.f : M1;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int r = 0; r < kMaxCluster; ++r) {
-            const float f0 = ex2(a[r].x - z0), f1 = ex2(b[r].x - z1);
-            L0 += a[r].y * f0;
-            L1 += b[r].y * f1;
-            x.x += v[r].x * f0;
-            x.y += v[r].y * f0;
-            x.z += v[r].z * f1;
-            x.w += v[r].w * f1;
-        }
-        const float i0 = L0 != 0.f ? 1.f / L0 : 0.f, i1 = L1 != 0.f ? 1.f / L1 : 0.f;
+        Joined j;
+        j.add(C, [&](int r, float2 &a, float2 &b, float4 &v) {
+            a = ld_cluster2(peer(&ml[ht * 16 + r0], r));
+            b = ld_cluster2(peer(&ml[ht * 16 + r0 + 8], r));
+            v = ld_cluster4(peer(&box[t * 32 + lane], r));
+        });
+        const float i0 = j.ml0.y != 0.f ? 1.f / j.ml0.y : 0.f, i1 = j.ml1.y != 0.f ? 1.f / j.ml1.y : 0.f;
         const int left = p.G - ht * 16;
         uint32_t *op = reinterpret_cast<uint32_t *>(
             static_cast<uint8_t *>(p.out) + ((item * p.G + ht * 16 + r0) * D + tile * 8 + (lane & 3) * 2) * 2);
-        if (r0 < left) op[0] = Num<T>::pack(x.x * i0, x.y * i0);
-        if (r0 + 8 < left) op[4 * D] = Num<T>::pack(x.z * i1, x.w * i1);
+        if (r0 < left) op[0] = Num<T>::pack(j.o.x * i0, j.o.y * i0);
+        if (r0 + 8 < left) op[4 * D] = Num<T>::pack(j.o.z * i1, j.o.w * i1);
         if (p.lse && tile == 0 && (lane & 3) == 0) {
             float *l = p.lse + item * p.G + ht * 16 + r0;
-            if (r0 < left) l[0] = L0 != 0.f ? (M0 + log2f(L0)) * kLn2 : -INFINITY;
-            if (r0 + 8 < left) l[8] = L1 != 0.f ? (M1 + log2f(L1)) * kLn2 : -INFINITY;
+            if (r0 < left) l[0] = lse2_of(j.ml0) * kLn2;
+            if (r0 + 8 < left) l[8] = lse2_of(j.ml1) * kLn2;
         }
     }
-    if (p.weights) {
-        if (tid < 16 * MT) {
-            float M = -INFINITY, L = 0.f;
-            float2 a[kMaxCluster];
-#pragma unroll
-            for (int r = 0; r < kMaxCluster; ++r) {
-                a[r] = r < C ? ld_cluster2(peer(&ml[tid], r)) : make_float2(-INFINITY, 0.f);
-                M = fmaxf(M, a[r].x);
-            }
-#pragma unroll
-            for (int r = 0; r < kMaxCluster; ++r) L += a[r].y * ex2(a[r].x - (M == -INFINITY ? 0.f : M));
-            z[tid] = L != 0.f ? M + log2f(L) : -INFINITY;
-        }
+    if (p.weights && tid < 16 * MT) {
+        Joined j;
+        j.add(C, [&](int r, float2 &a, float2 &, float4 &) { a = ld_cluster2(peer(&ml[tid], r)); });
+        z[tid] = lse2_of(j.ml0);
     }
     __syncwarp();
     cluster_arrive();
@@ -375,8 +404,10 @@ template <int MT> __device__ __forceinline__ void team_sync(int team) {
 
 // kNear: a cluster has one item and joins it itself.
 template <typename T, int D, int MT, bool kNear>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __grid_constant__ Params p) {
-    using S = Shape<D, MT>;
+__global__ void __launch_bounds__(Shape<D, MT, kNear>::kThreads, kNear ? 1 : kBlocksPerSm)
+    attend_kernel(const __grid_constant__ Params p) {
+    using S = Shape<D, MT, kNear>;
+    constexpr int kWarps = S::kWarps, kThreads = S::kThreads;
     constexpr int kTeams = S::kTeams, kStep = S::kStep, kSlots = S::kSlots, kRow = S::kRow, kUnit = S::kUnit;
     constexpr uint32_t kHalf = S::kHalf, kSlot = S::kSlot;
     constexpr int kLanes = kRow / 16, kRows = 32 / kLanes;  // lanes of a row, rows of one copy instruction
@@ -593,7 +624,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
                     x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, i));
                     x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, i));
                 }
-                if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
+                // The maximum taken out may stay behind the true one by up to 2^kLag: probabilities up to that are held as
+                // well, and the output is rescaled that much more rarely.
+                if (__any_sync(0xffffffffu, x0 > m0 + kLag || x1 > m1 + kLag)) {
                     x0 = fmaxf(x0, m0);
                     x1 = fmaxf(x1, m1);
                     const float a0 = x0 == -INFINITY ? 1.f : ex2(m0 - x0), a1 = x1 == -INFINITY ? 1.f : ex2(m1 - x1);
@@ -639,8 +672,12 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
             l0 += __shfl_xor_sync(0xffffffffu, l0, i);
             l1 += __shfl_xor_sync(0xffffffffu, l1, i);
         }
+        if constexpr (kNear) {
+            join_cluster<T, D, MT>(p, o, make_float2(m0, l0), make_float2(m1, l1), item, C, rank, u0, u1, at.len, smem);
+            return;
+        }
         // the first team takes in what the others leave, half of the columns at a time
-        if constexpr (kTeams > 1) {
+        if constexpr (!kNear && kTeams > 1) {
             if (team > 0 && (lane & 3) == 0) {
                 merge_ml[warp - MT][r0] = make_float2(m0, l0);
                 merge_ml[warp - MT][r0 + 8] = make_float2(m1, l1);
@@ -700,10 +737,6 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const __
                 }
                 __syncthreads();
             }
-        }
-        if constexpr (kNear) {
-            join_cluster<T, D, MT>(p, o, make_float2(m0, l0), make_float2(m1, l1), item, C, rank, u0, u1, at.len, smem);
-            return;
         }
         if (team == 0) {
             if (from_start && to_end) {  // the whole item
@@ -888,39 +921,58 @@ Layout layout_of(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t max_len, 
     return l;
 }
 
-// Blocks of a cluster that has one item, or 0 where the work is dealt out evenly instead.  A cluster joins its item itself,
-// without a second kernel, but its blocks idle where other sequences are longer: it pays where every item at its longest
-// is short work for its blocks and all are resident at once.
-int cluster_for(const Params &p, int64_t D, int64_t unit) {
-    const int64_t units = ((int64_t)p.max_len + unit - 1) / unit, items = (int64_t)p.B * p.Hk;
-    int64_t C = 1;
-    while (C < kMaxCluster && C < units && items * C * 2 <= workers_of_device()) C *= 2;
-    return items * C <= workers_of_device() && (units + C - 1) / C * unit * D <= kNearWork ? (int)C : 0;
+// Clusters of 2^i blocks of a kernel that are resident at once on the current device.
+int active_clusters(const void *kernel, cudaLaunchConfig_t &cfg, std::atomic<int32_t> (&known)[kMaxDevices][5], int i) {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= kMaxDevices) return 0;
+    if (const int have = known[dev][i].load(std::memory_order_relaxed)) return have - 1;
+    cfg.attrs[0].val.clusterDim.x = 1u << i;
+    cfg.gridDim = dim3(1u << i);
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n = 0;
+    }
+    known[dev][i].store(n + 1, std::memory_order_relaxed);
+    return n;
 }
 
 template <typename T, int D, int MT> int launch(const Params &p, cudaStream_t s) {
-    constexpr uint32_t smem = Shape<D, MT>::kSmem;
     const int64_t items = (int64_t)p.B * p.Hk;
-    if (const int C = cluster_for(p, D, Shape<D, MT>::kUnit)) {
+    {
+        // A cluster that has one item joins it itself, without a second kernel, but its blocks idle where other sequences
+        // are longer: it pays where every item at its longest is short work for its blocks, and all are resident at once.
+        using S = Shape<D, MT, true>;
         auto *kernel = attend_kernel<T, D, MT, true>;
-        UNUM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        static std::atomic<int32_t> known[kMaxDevices][5];
+        UNUM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
+        UNUM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)(items * C));
-        cfg.blockDim = dim3(kThreads);
-        cfg.dynamicSmemBytes = smem;
+        cfg.blockDim = dim3(S::kThreads);
+        cfg.dynamicSmemBytes = S::kSmem;
         cfg.stream = s;
         cudaLaunchAttribute attr = {};
         attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = (unsigned)C;
         attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
-        UNUM_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
-        return unum::check_launch("attend_kernel");
+        const int64_t units = ((int64_t)p.max_len + S::kUnit - 1) / S::kUnit;
+        int i = 0;
+        while ((2 << i) <= kMaxCluster && (1 << i) < units &&
+               items <= active_clusters((const void *)kernel, cfg, known, i + 1))
+            ++i;
+        const int64_t C = 1 << i;
+        if (items <= active_clusters((const void *)kernel, cfg, known, i) &&
+            (units + C - 1) / C * S::kUnit * D <= kNearWork) {
+            cfg.gridDim = dim3((unsigned)(items * C));
+            attr.val.clusterDim.x = (unsigned)C;
+            UNUM_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+            return unum::check_launch("attend_kernel");
+        }
     }
     auto *kernel = attend_kernel<T, D, MT, false>;
+    constexpr uint32_t smem = Shape<D, MT, false>::kSmem;
     UNUM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    kernel<<<(unsigned)p.workers, kThreads, smem, s>>>(p);
+    kernel<<<(unsigned)p.workers, Shape<D, MT, false>::kThreads, smem, s>>>(p);
     if (int rc = unum::check_launch("attend_kernel")) return rc;
     // A long item is cut into about workers / items parts, and then a block of the second kernel has one tile's columns
     // and 16 warps on its parts; where items are many they have a few parts each, and a block has the whole row.
