@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
 //            one (mostly the third for long sequences, the second or third for short ones).  (Adding them up with remote atomics took 13 us a digit with 16
 //            blocks: they are served one at a time.)
 //   write    each warp has a contiguous part of the slice; a count and one scan over the warps give each page its
-//            place, among those that stay or among the evicted, and the weights move along, 128 pages at a time.
+//            place, among those that stay or among the evicted, and the weights move along.
 // What is filled behind the new ends does not wait for any of it and is written first.
 // Bound by latency for one sequence (the barriers), by HBM for a batch.
 constexpr int kEvThreads = 512;  // with 1024, block barriers cost more than the added warps hid (12.5 against 10.3 us)
@@ -71,7 +71,7 @@ constexpr int64_t kMaxPages = kMaxCluster * kMaxSlice;
 constexpr int kBins = 256;
 constexpr int kGroups = kEvThreads / kBins;
 constexpr int kCopies = 8;   // of the histogram
-constexpr int kBatch = 4;    // loads of a thread under way, and 32-page chunks of a warp's write step
+constexpr int kBatch = 4;    // loads of a thread under way
 
 struct EvictParams {
     const int32_t *table, *seqlens;
@@ -143,7 +143,6 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
     __shared__ uint32_t warp_sums[kEvWarps];
     __shared__ uint32_t found[3];    // the digit, how many are still wanted with it, and how many have it
     __shared__ uint32_t slice_eq, slice_sure;
-    __shared__ int32_t list[kEvWarps][32 * kBatch];  // of a warp's pages in hand those that stay
     const uint32_t rank = cluster_rank(), C = cluster_size();
     const int64_t b = blockIdx.x / C;
     const int32_t P = 1 << p.shift;
@@ -350,46 +349,44 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
         edge = prefix;
         edge_from = all_from;
     }
-    // places, and the weights of the pages that stay
-    for (int32_t j0 = i0; j0 < i1; j0 += 32 * kBatch) {
+    // places.  The warp's list of pages that stay takes the room of its keys, behind where it reads.
+    const int64_t to = (kept_before + stay_at) << p.shift;
+    int32_t m = 0, page = i0 + lane < i1 ? __ldg(trow + s0 + i0 + lane) : 0;
+#pragma unroll 1
+    for (int32_t j0 = i0; j0 < i1; j0 += 32) {
+        const int32_t i = j0 + lane, my_page = page;
+        if (i + 32 < i1) page = __ldg(trow + s0 + i + 32);
         const uint32_t below = (1u << lane) - 1;
-        int32_t page[kBatch], m = 0;
-#pragma unroll
-        for (int e = 0; e < kBatch; ++e)
-            if (j0 + 32 * e + lane < i1) page[e] = __ldg(trow + s0 + j0 + 32 * e + lane);
-#pragma unroll
-        for (int e = 0; e < kBatch; ++e) {
-            const int32_t i = j0 + 32 * e + lane;
-            bool stay = i < i1;
-            if (drop > 0) {
-                const uint32_t key = stay ? keys[i] : 0;
-                const bool sure = stay && (i < cand0 || i >= cand1 || key >= edge_from);
-                const bool eq = stay && !sure && key == edge;
-                const uint32_t eqs = __ballot_sync(0xffffffffu, eq);
-                stay = sure || (eq && eq_at + __popc(eqs & below) < eq_left);
-                eq_at += __popc(eqs);
-            }
-            const uint32_t stays = __ballot_sync(0xffffffffu, stay);
-            const int32_t at = m + __popc(stays & below);
-            if (stay) {
-                nrow[kept_before + stay_at + at] = page[e];
-                list[warp][at] = i;
-            } else if (i < i1) {
-                erow[s0 + i - kept_before - stay_at - at] = page[e];
-            }
-            m += __popc(stays);
+        bool stay = i < i1;
+        if (drop > 0) {
+            const uint32_t key = stay ? keys[i] : 0;
+            const bool sure = stay && (i < cand0 || i >= cand1 || key >= edge_from);
+            const bool eq = stay && !sure && key == edge;
+            const uint32_t eqs = __ballot_sync(0xffffffffu, eq);
+            stay = sure || (eq && eq_at + __popc(eqs & below) < eq_left);
+            eq_at += __popc(eqs);
         }
-        __syncwarp();
-        const int64_t to = (kept_before + stay_at) << p.shift;
-        stay_at += m;
-        m <<= p.shift;
+        const uint32_t stays = __ballot_sync(0xffffffffu, stay);
+        const int32_t at = m + __popc(stays & below);
+        if (stay) {
+            nrow[kept_before + stay_at + at] = my_page;
+            keys[i0 + at] = (uint32_t)i;
+        } else if (i < i1) {
+            erow[s0 + i - kept_before - stay_at - at] = my_page;
+        }
+        m += __popc(stays);
+    }
+    __syncwarp();
+    // and the weights of those pages
+    m <<= p.shift;
+    {
         constexpr int kWide = kVec ? 4 : 1;
         for (int32_t q0 = lane * kWide; q0 < m; q0 += 32 * kWide * kBatch) {
             int64_t from[kBatch];
 #pragma unroll
             for (int e = 0; e < kBatch; ++e) {
                 const int32_t q = q0 + 32 * kWide * e;
-                from[e] = q < m ? ((s0 + list[warp][q >> p.shift]) << p.shift) + (q & (P - 1)) : len;
+                from[e] = q < m ? ((s0 + keys[i0 + (q >> p.shift)]) << p.shift) + (q & (P - 1)) : len;
             }
 #pragma unroll 2
             for (int32_t h = 0; h < p.Hk; ++h) {
@@ -419,7 +416,6 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
                 }
             }
         }
-        __syncwarp();
     }
     if (rank == 0 && tid == 0) p.new_lens[b] = (int32_t)(len - (drop << p.shift));
     if (drop > 0 && C > 1) cluster_wait();
