@@ -384,7 +384,8 @@ int unum_compress_keys(const void *k, int64_t T, int64_t Hk, int64_t D, int64_t 
 
 /*
  * cache_append — writes new tokens' keys and values to their places.
- *   k, v     [T, Hk, D] of the cache's 2-byte type (strides in elements, multiples of 8; 16-byte aligned)
+ *   k, v     [T, Hk, D] of the cache's 2-byte type (strides in elements, multiples of 8; 16-byte aligned), apart
+ *            from the caches
  *   token_to_bs, token_pos_in_bs  int32 [T]: token t is position token_pos_in_bs[t] - 1 of its sequence (the last
  *            of the positions it sees, as for unum_get_block_table)
  * A token whose sequence is outside [0, B), whose position is outside the table or whose table entry is not held
@@ -429,7 +430,7 @@ int unum_paged_attention(const void *q, int64_t B, int64_t Hq, int64_t D, int64_
  *   new_seqlens int32 [B]: less page_size for each evicted page
  *   new_weights float [B, Hk, n_pages * page_size]: moved along with their pages, 0 behind the new length
  *   evicted     int32 [B, n_pages]: the evicted entries in their order, then -1
- * The outputs must not overlap the inputs.  n_pages <= 409600 and n_pages * page_size < 2^31.
+ * The outputs must not overlap the inputs.  n_pages <= 409600 and n_pages * page_size < 2^30.
  */
 int unum_cache_evict(const int32_t *block_table, int64_t B, int64_t n_pages, int64_t bt_stride,
                      const int32_t *seqlens, const float *weights, int64_t Hk, int64_t w_sb, int64_t w_sh,

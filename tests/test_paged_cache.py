@@ -203,7 +203,7 @@ def test_cpu_tensors_are_refused(lib):
     with pytest.raises(ValueError, match="CUDA"):
         paged_attention(q, kc, vc, table, lens)
     with pytest.raises(ValueError, match="CUDA"):
-        append_cache(kc[:2], vc[:2], kc, vc, table, lens, lens)
+        append_cache(kc[:2].clone(), vc[:2].clone(), kc, vc, table, lens, lens)
     with pytest.raises(ValueError, match="CUDA"):
         evict_cache(table, lens, torch.zeros(2, 2, table.shape[1]), budget=4)
 
@@ -238,6 +238,13 @@ def test_append_and_evict_wrappers_refuse(lib):
 
     _, kc, vc, table, lens = make_case(1, [5, 9], 2, 4, 64, 1, "bf16")
     k, i = kc[:2].clone(), torch.zeros(2, dtype=torch.int32)
+    for a in [(kc[3:5], k, kc, vc), (k, vc[-2:], kc, vc)]:
+        with pytest.raises(ValueError, match="memory"):
+            append_cache(*a, table, i, i)
+    with pytest.raises(TypeError):
+        append_cache(k, [1], kc, vc, table, i, i)
+    with pytest.raises(TypeError):
+        append_cache(k, k, kc, vc, table, i, i, page_size=1.5)
     for a in [(k.float(), k, kc, vc), (k[:, :1], k[:, :1], kc, vc), (k, k[:1], kc, vc), (k, k, kc, kc),
               (k, k, kc[:1].expand(12, 2, 64), vc[:12]), (k, k, kc[:, :1].expand(-1, 2, -1), vc)]:
         with pytest.raises(ValueError):
@@ -279,6 +286,50 @@ def test_attention(lens, Hk, G, D, page, dtype, gather):
         before = torch.from_numpy(np.random.default_rng(5).random((len(lens), Hk, table.shape[1] * page)).astype(np.float32))
     out, lse, after = run_attention(q, kc, vc, table, ln, page, before)
     check_attention(q, kc, vc, table, ln, page, D ** -0.5, out, lse, before, after)
+
+
+# Work that is dealt out in units and joined by the second kernel: more than the clusters take.
+DEALT = [
+    ([20000], 2, 16, 128, 1, "bf16"), ([40000, 5, 0, 1300], 1, 8, 64, 16, "fp16"), ([1500, 3, 0, 2000] + [700] * 40, 2, 32, 128, 64, "bf16"),
+    ([17000, 4000], 2, 64, 128, 2, "bf16"), ([33000, 1], 1, 33, 64, 128, "fp16"), ([100] * 200, 2, 5, 128, 4, "bf16"),
+    ([0] * 150 + [65, 0, 64, 1, 0, 129, 3000], 2, 16, 128, 1, "fp16"), ([70000], 1, 1, 64, 1, "bf16"), ([12345] * 3, 4, 20, 64, 32, "bf16"),
+    (list(range(0, 900, 3)), 1, 16, 128, 16, "bf16"), ([31, 33] * 80, 1, 40, 128, 8, "fp16"),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,Hk,G,D,page,dtype", DEALT)
+@pytest.mark.parametrize("gather", [False, True])
+def test_attention_dealt_out(lens, Hk, G, D, page, dtype, gather):
+    test_attention(lens, Hk, G, D, page, dtype, gather)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bound", [1000, 1024, 1025, 5000, 16384, 16385, 30000])
+def test_attention_the_bound_of_the_lengths_changes_the_split_only(bound):
+    """The same sequences under several host-side bounds (each another split of the work), all within tolerance."""
+    lens = [1000, 999, 0, 513]
+    q, kc, vc, table, ln = make_case(31, lens, 2, 16, 128, 1, "bf16", spare=bound - 1000)
+    before = torch.rand(4, 2, table.shape[1], generator=torch.Generator().manual_seed(2))
+    out, lse, after = run_attention(q, kc, vc, table, ln, 1, before, max_seqlen=bound)
+    check_attention(q, kc, vc, table, ln, 1, 128 ** -0.5, out, lse, before, after)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [2, 200])
+def test_attention_over_nothing(B):
+    """A table without a page, a cache without a token, a batch without a sequence."""
+    from unum_ops_b200 import paged_attention
+
+    d = dev()
+    q, kc = torch.randn(B, 32, 128, device=d, dtype=torch.bfloat16), torch.randn(9, 2, 128, device=d, dtype=torch.bfloat16)
+    i32 = dict(dtype=torch.int32, device=d)
+    for k, table in ((kc, torch.zeros(B, 0, **i32)), (kc[:0], torch.zeros(B, 7, **i32))):
+        w = torch.ones(B, 2, 7, device=d)
+        out, lse = paged_attention(q, k, k, table, torch.full((B,), 5, **i32), weights=w, return_lse=True)
+        assert not out.any() and torch.isneginf(lse).all() and (w == 1).all()
+    out = paged_attention(q[:0], kc, kc, torch.zeros(0, 3, **i32), torch.zeros(0, **i32))
+    assert out.shape == (0, 32, 128)
 
 
 @pytest.mark.gpu
@@ -380,13 +431,14 @@ def test_attention_offsets_past_32_bits():
 
 
 @pytest.mark.gpu
-def test_attention_same_bits_again_and_in_a_graph():
+@pytest.mark.parametrize("lens", [[3000, 40, 0, 1777], [30000, 40, 0, 17771]])
+def test_attention_same_bits_again_and_in_a_graph(lens):
     """Two calls give the same bits; a captured call follows its inputs; two graphs replayed on two streams at once do not
     share a workspace."""
     import unum_ops_b200
 
     d = dev()
-    q, kc, vc, table, ln = [x.to(d) for x in make_case(12, [3000, 40, 0, 1777], 2, 16, 128, 1, "bf16")]
+    q, kc, vc, table, ln = [x.to(d) for x in make_case(12, lens, 2, 16, 128, 1, "bf16")]
     w = torch.zeros(4, 2, table.shape[1], device=d)
     call = lambda: unum_ops_b200.paged_attention(q, kc, vc, table, ln, weights=w, return_lse=True)  # noqa: E731
     a, la = call()

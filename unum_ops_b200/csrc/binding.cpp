@@ -131,6 +131,19 @@ bool overlaps(const Tensor &t) {
     return false;
 }
 
+// Whether the stretches of memory that two tensors span meet.
+bool meet(const Tensor &a, const Tensor &b) {
+    if (a.numel() == 0 || b.numel() == 0) return false;
+    auto span = [](const Tensor &t) {
+        int64_t last = 0;
+        for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+        const uintptr_t at = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+        return std::make_pair(at, at + (last + 1) * t.element_size());
+    };
+    const auto x = span(a), y = span(b);
+    return x.first < y.second && y.first < x.second;
+}
+
 Tensor as_i32(const Tensor &t) { return (t.scalar_type() == at::kInt ? t : t.to(at::kInt)).contiguous(); }
 
 void check_cache(const Tensor &k, const Tensor &v) {
@@ -180,6 +193,8 @@ PyObject *append_cache(const Args &a) {
                v.scalar_type());
     if (overlaps(kc) || overlaps(vc) || (kc.numel() && kc.const_data_ptr() == vc.const_data_ptr()))
         refuse(PyExc_ValueError, "k_cache and v_cache are written to: their rows must not share memory");
+    if (meet(k, kc) || meet(k, vc) || meet(v, kc) || meet(v, vc))
+        refuse(PyExc_ValueError, "k and v must not lie in the memory of k_cache and v_cache");
     const int64_t T = k.size(0);
     if (bs.numel() != T || pos.numel() != T)
         refuse(PyExc_ValueError, "token_to_bs and token_pos_in_bs must have one entry for each of ", T, " tokens; got ",

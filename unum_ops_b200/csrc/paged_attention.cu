@@ -73,6 +73,25 @@ struct Params {
 // ---------------------------------------------------------------------------------------------- instructions
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
+__device__ __forceinline__ uint64_t evict_first() {
+    uint64_t policy;
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
+__device__ __forceinline__ uint64_t evict_last() {
+    uint64_t policy;
+    asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
+__device__ __forceinline__ void st_hint(float *p, float x, float y, uint64_t policy) {
+    asm volatile("st.global.L2::cache_hint.v2.f32 [%0], {%1, %2}, %3;" ::"l"(p), "f"(x), "f"(y), "l"(policy) : "memory");
+}
+__device__ __forceinline__ float4 ld_hint(const float *p, uint64_t policy) {
+    float4 v;
+    asm volatile("ld.global.L1::no_allocate.L2::cache_hint.v4.f32 {%0, %1, %2, %3}, [%4], %5;"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p), "l"(policy) : "memory");
+    return v;
+}
 // 16 zero bytes where `bytes` is 0
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes, uint64_t policy) {
     asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(bytes),
@@ -81,11 +100,6 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32
 }
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void *src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ uint64_t evict_first() {
-    uint64_t policy;
-    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-    return policy;
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -259,6 +273,7 @@ __device__ __forceinline__ void gather4(const Params &p, int64_t item, const flo
     const float *sc = p.scores + item * p.G * p.score_ld + pos;
     // positions not held have a score of -inf: they gather nothing, even where the head's lse is NaN
     auto term = [](float s, float zh) { return s == -INFINITY || zh == -INFINITY ? 0.f : ex2(s - zh); };
+    const uint64_t policy = evict_first();  // read once: what was kept for this makes room
     float old[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -266,7 +281,7 @@ __device__ __forceinline__ void gather4(const Params &p, int64_t item, const flo
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
     for (int h = 0; h < p.G; ++h) {
-        const float4 s = __ldcs(reinterpret_cast<const float4 *>(sc + h * p.score_ld));
+        const float4 s = ld_hint(sc + h * p.score_ld, policy);
         const float zh = z[h];
         x.x += term(s.x, zh);
         x.y += term(s.y, zh);
@@ -495,9 +510,9 @@ __global__ void __launch_bounds__(Shape<D, MT, kNear>::kThreads, kNear ? 1 : kBl
     const int copy_row = ht * kRows + lane / kLanes;
     const uint32_t copy_to = ring + copy_row * kRow;
     const uint32_t copy_chunk = lane % kLanes;
-    // The cache passes through L2 once and makes room first: what the second kernel reads stays (group 32 with weights
-    // 55.3 -> 51.4 us; 131072 positions 39.3 -> 38.0 us).
-    const uint64_t policy = evict_first();
+    // The cache passes through L2 once and makes room first, the scores stay until they are read (24 sequences of 2048 to
+    // 32768 with weights: 101.6 us with the hint on the cache alone, 97.3 us with both).
+    const uint64_t policy = evict_first(), keep = evict_last();
     auto issue = [&](uint32_t slot) {
         const int2 step = ahead[warp][slot];
         const int64_t page = entries[slot * kStep];
@@ -605,10 +620,9 @@ __global__ void __launch_bounds__(Shape<D, MT, kNear>::kThreads, kNear ? 1 : kBl
 #pragma unroll
                         for (int t = 0; t < kStep / 8; ++t) {
                             if (ht * 16 + r0 < p.G)
-                                *reinterpret_cast<float2 *>(sc + pos + 8 * t) = make_float2(s[t][0], s[t][1]);
+                                st_hint(sc + pos + 8 * t, s[t][0], s[t][1], keep);
                             if (ht * 16 + r0 + 8 < p.G)
-                                *reinterpret_cast<float2 *>(sc + 8 * p.score_ld + pos + 8 * t) =
-                                    make_float2(s[t][2], s[t][3]);
+                                st_hint(sc + 8 * p.score_ld + pos + 8 * t, s[t][2], s[t][3], keep);
                         }
                     }
                     if (mask == 0) continue;

@@ -496,7 +496,7 @@ extern "C" int unum_cache_evict(const int32_t *block_table, int64_t B, int64_t n
         unum::set_error("at most %lld pages a sequence (got %lld)", (long long)kMaxPages, (long long)n_pages);
         return UNUM_ERR_UNSUPPORTED;
     }
-    UNUM_CHECK_ARG(n_pages * page_size < ((int64_t)1 << 31), "n_pages * page_size must stay below 2^31");
+    UNUM_CHECK_ARG(n_pages * page_size < ((int64_t)1 << 30), "n_pages * page_size must stay below 2^30");
     UNUM_CHECK_ARG(B < ((int64_t)1 << 28), "too many sequences");
     UNUM_CHECK_ARG(seqlens && new_seqlens, "null pointer argument");
     UNUM_CHECK_ARG(n_pages == 0 || (block_table && weights && new_table && new_weights && evicted),

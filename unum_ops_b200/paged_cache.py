@@ -26,7 +26,7 @@ __all__ = ["append_cache", "paged_attention", "evict_cache"]
 def append_cache(k, v, k_cache, v_cache, block_table, token_to_bs, token_pos_in_bs, *, page_size=1):
     """Write new tokens' keys and values to their places in the cache, in place.
 
-    k, v             [T, Hk, D] of the cache's dtype (any strides)
+    k, v             [T, Hk, D] of the cache's dtype (any strides), not in the caches' memory
     block_table      int32 [B, n_pages]
     token_to_bs      int32 [T], the tokens' sequences
     token_pos_in_bs  int32 [T], as for get_block_table: token t sees that many positions,
@@ -81,5 +81,5 @@ def evict_cache(block_table, seqlens, weights, *, budget, init_pages=0, local_pa
         weights      moved along with their pages, 0 behind the new lengths
         evicted      int32 [B, n_pages]: the evicted entries in their order, then -1: what the
                      caller's allocator gets back
-    Keys and values stay where they are."""
+    Keys and values stay where they are.  At most 409600 pages a sequence."""
     return _lib.binding().evict_cache(block_table, seqlens, weights, budget, init_pages, local_pages, page_size)
