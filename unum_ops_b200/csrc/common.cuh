@@ -51,4 +51,22 @@ inline int sm_count() {
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Programmatic dependent launch: a kernel launched with this attribute may start while the one before it in the stream
+// still runs, so that its launch is not waited for.  Such a kernel begins with wait_for_previous_kernel in every thread,
+// before it reads or writes anything and before any block ends: it returns when everything before has completed and is
+// visible, and from then on lets the kernel behind it start in the same way.
+inline cudaLaunchAttribute behind_previous_kernel() {
+    cudaLaunchAttribute a = {};
+    a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a.val.programmaticStreamSerializationAllowed = 1;
+    return a;
+}
+
+#ifdef __CUDACC__
+__device__ __forceinline__ void wait_for_previous_kernel() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+#endif
+
 }  // namespace unum

@@ -438,6 +438,8 @@ __global__ void __launch_bounds__(Shape<D, MT, kNear>::kThreads, kNear ? 1 : kBl
     float4 *merge = reinterpret_cast<float4 *>(smem + S::kMergeAt);
     int32_t *entries = reinterpret_cast<int32_t *>(smem + S::kEntriesAt) + warp * (kSlots * kStep) + (lane & (kStep - 1));
 
+    // Launched while the kernel before it may still run, and lets the one behind it do so.
+    unum::wait_for_previous_kernel();
     const int32_t C = kNear ? cluster_size() : 1, rank = kNear ? cluster_rank() : 0, me = blockIdx.x;
     int32_t u0, u1;
     Place<kUnit> in;  // where the entries are read
@@ -455,7 +457,6 @@ __global__ void __launch_bounds__(Shape<D, MT, kNear>::kThreads, kNear ? 1 : kBl
         u0 = in.unit = shares.begin(rank);
         u1 = shares.begin(rank + 1);
     } else {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // this block's share of the units
     const int32_t per = (p.B + kThreads - 1) / kThreads;
     const int32_t b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
@@ -805,7 +806,7 @@ __global__ void __launch_bounds__(kJoinThreads, 2) join_kernel(const __grid_cons
     __shared__ float2 ml[kMaxWorkers][17];  // of each part and head: maximum and sum.  17: banks
     __shared__ float4 sums[kJoinWarps][32];
     __shared__ __align__(16) float z[kMaxG];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    unum::wait_for_previous_kernel();
     const int32_t item = blockIdx.x, b = item / p.Hk, g = item - b * p.Hk;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int32_t len = length(p, b);
@@ -964,11 +965,12 @@ template <typename T, int D, int MT> int launch(const Params &p, cudaStream_t s)
         cfg.blockDim = dim3(S::kThreads);
         cfg.dynamicSmemBytes = S::kSmem;
         cfg.stream = s;
-        cudaLaunchAttribute attr = {};
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
+        cudaLaunchAttribute attr[2] = {};
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1] = unum::behind_previous_kernel();
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;  // what the occupancy takes
         const int64_t units = ((int64_t)p.max_len + S::kUnit - 1) / S::kUnit;
         int i = 0;
         while ((2 << i) <= kMaxCluster && (1 << i) < units &&
@@ -978,7 +980,8 @@ template <typename T, int D, int MT> int launch(const Params &p, cudaStream_t s)
         if (items <= active_clusters((const void *)kernel, cfg, known, i) &&
             (units + C - 1) / C * S::kUnit * D <= kNearWork) {
             cfg.gridDim = dim3((unsigned)(items * C));
-            attr.val.clusterDim.x = (unsigned)C;
+            attr[0].val.clusterDim.x = (unsigned)C;
+            cfg.numAttrs = 2;
             UNUM_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
             return unum::check_launch("attend_kernel");
         }
@@ -986,8 +989,15 @@ template <typename T, int D, int MT> int launch(const Params &p, cudaStream_t s)
     auto *kernel = attend_kernel<T, D, MT, false>;
     constexpr uint32_t smem = Shape<D, MT, false>::kSmem;
     UNUM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    kernel<<<(unsigned)p.workers, Shape<D, MT, false>::kThreads, smem, s>>>(p);
-    if (int rc = unum::check_launch("attend_kernel")) return rc;
+    cudaLaunchAttribute attr = unum::behind_previous_kernel();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.workers);
+    cfg.blockDim = dim3(Shape<D, MT, false>::kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    UNUM_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
     // A long item is cut into about workers / items parts, and then a block of the second kernel has one tile's columns
     // and 16 warps on its parts; where items are many they have a few parts each, and a block has the whole row.
     int tiles = D / 8;
@@ -999,15 +1009,9 @@ template <typename T, int D, int MT> int launch(const Params &p, cudaStream_t s)
         const int64_t most = ((int64_t)p.max_len + 4 * kJoinThreads - 1) / (4 * kJoinThreads);
         if (gather > most) gather = most;
     }
-    cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)items, (unsigned)(splits + gather));
     cfg.blockDim = dim3(kJoinThreads);
-    cfg.stream = s;
-    cudaLaunchAttribute attr = {};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cfg.dynamicSmemBytes = 0;
     UNUM_CHECK_CUDA(cudaLaunchKernelEx(&cfg, join_kernel<T, D, MT>, p, (int32_t)tiles, (int32_t)splits));
     return unum::check_launch("join_kernel");
 }

@@ -34,6 +34,7 @@ struct AppendParams {
 };
 
 __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendParams p) {
+    unum::wait_for_previous_kernel();
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t t = i / p.chunks;
     if (t >= p.T) return;
@@ -143,6 +144,7 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
     __shared__ uint32_t warp_sums[kEvWarps];
     __shared__ uint32_t found[3];    // the digit, how many are still wanted with it, and how many have it
     __shared__ uint32_t slice_eq, slice_sure;
+    unum::wait_for_previous_kernel();
     const uint32_t rank = cluster_rank(), C = cluster_size();
     const int64_t b = blockIdx.x / C;
     const int32_t P = 1 << p.shift;
@@ -473,7 +475,14 @@ extern "C" int unum_cache_append(const void *k, const void *v, int64_t T, int64_
     p.chunks = (int32_t)(Hk * (D / 8));
     const int64_t blocks = (T * p.chunks + 255) / 256;
     UNUM_CHECK_ARG(T < ((int64_t)1 << 40) && blocks < ((int64_t)1 << 31), "too many tokens");
-    append_kernel<<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(p);
+    cudaLaunchAttribute attr = unum::behind_previous_kernel();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(256);
+    cfg.stream = (cudaStream_t)stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    UNUM_CHECK_CUDA(cudaLaunchKernelEx(&cfg, append_kernel, p));
     return unum::check_launch("append_kernel");
 }
 
@@ -536,12 +545,13 @@ extern "C" int unum_cache_evict(const int32_t *block_table, int64_t B, int64_t n
     cfg.blockDim = dim3(kEvThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute attr = {};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = (unsigned)C;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)C;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1] = unum::behind_previous_kernel();
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
     UNUM_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
     return unum::check_launch("evict_kernel");
 }
