@@ -471,6 +471,52 @@ def test_attention_same_bits_again_and_in_a_graph(lens):
         assert torch.equal(o, want) and torch.equal(l, wl) and torch.equal(weights, fresh)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[500, 40, 0, 177], [30000, 40, 0, 17771]])
+def test_calls_behind_kernels_that_still_run(lens):
+    """Kernels are launched while the one before them runs: what that one writes (q, the cache, the lengths, the table)
+    is waited for, and so is what the calls themselves leave for the next kernel.  No synchronisation inside."""
+    from unum_ops_b200 import append_cache, evict_cache, paged_attention
+
+    d = dev()
+    q, kc, vc, table, ln = [x.to(d) for x in make_case(14, lens, 2, 16, 128, 1, "bf16")]
+    W = table.shape[1]
+    slow = torch.randn(3000, 3000, device=d)
+    want = paged_attention(q, kc, vc, table, ln, return_lse=True)
+    w = torch.rand(4, 2, W, device=d)
+    want_evicted = evict_cache(table, ln, w, budget=100)
+    k, v = torch.randn(2, 300, 2, 128, device=d, dtype=torch.bfloat16)
+    rows = torch.arange(300, device=d, dtype=torch.int32)
+    torch.cuda.synchronize()
+    for _ in range(4):
+        q2, k2, t2, l2, w2 = torch.zeros_like(q), torch.zeros_like(kc), torch.zeros_like(table), torch.zeros_like(ln), torch.zeros_like(w)
+        vc2, got = torch.full_like(vc, 9), []
+        torch.mm(slow, slow)
+        t2.copy_(table)
+        l2.copy_(ln)
+        w2.copy_(w)
+        q2.copy_(q)
+        vc2.copy_(vc)
+        k2.copy_(kc)  # the last and the largest: still running when the call is made
+        got.append(paged_attention(q2, k2, vc2, t2, l2, return_lse=True))
+        w2.mul_(1.0)
+        got.append(evict_cache(t2, l2, w2, budget=100))
+        first, n = got[1][0], got[1][1]
+        got.append(paged_attention(q2, k2, vc2, first, n, return_lse=True))
+        append_cache(k, v, k2, vc2, rows[None].expand(1, -1), torch.zeros_like(rows), rows + 1)
+        got.append((k2[:300].clone(), vc2[:300].clone()))
+        got.append(paged_attention(q2, k2, vc2, t2, l2, return_lse=True))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got[0], want))
+        assert all(torch.equal(a, b) for a, b in zip(got[1], want_evicted))
+        shorter = paged_attention(q, kc, vc, want_evicted[0], want_evicted[1], return_lse=True)
+        assert all(torch.equal(a, b) for a, b in zip(got[2], shorter))
+        assert torch.equal(got[3][0], k) and torch.equal(got[3][1], v)
+        kc3, vc3 = kc.clone(), vc.clone()
+        kc3[:300], vc3[:300] = k, v
+        assert all(torch.equal(a, b) for a, b in zip(got[4], paged_attention(q, kc3, vc3, table, ln, return_lse=True)))
+
+
 # ------------------------------------------------------------------------------------------------ append (GPU)
 @pytest.mark.gpu
 @pytest.mark.parametrize("T,B,Hk,D,page,dtype", [(1, 1, 2, 128, 1, "bf16"), (7, 3, 1, 64, 4, "fp16"), (500, 5, 8, 64, 16, "bf16"),
