@@ -9,21 +9,28 @@
 // A row without a valid position is 0 with lse = -inf.
 //
 // What bounds it: each key and value row is read once, 4 * D bytes a position and kv head, against 4 * D * G operations:
-// at G = 16 and HBM's full rate 100 TFLOP/s, 6% of the tensor cores.  So everything serves the loads:
-//   - work is split over the length in units of 64 positions.  The units of all (sequence, kv head) items, in a row,
-//     are dealt to the resident blocks in equal shares (two blocks an SM, one wave), so a batch of any lengths, one
+// at G = 16 and HBM's full rate 100 TFLOP/s, 6% of the tensor cores' rate.  So everything serves the loads:
+//   - work is split over the length in units of 64 or 128 positions.  The units of all (sequence, kv head) items, in a
+//     row, are dealt to the resident blocks in equal shares (two blocks an SM, one wave), so a batch of any lengths, one
 //     long sequence or many short ones, loads every SM alike;
-//   - a block's four warps take 16 positions of a unit each.  A warp (a team of 2 or 4 warps where G > 16: one for
-//     each 16 heads) has a ring of its own in shared memory, filled by 16-byte asynchronous copies that gather rows by
-//     the table, whose entries are read one step ahead.  No block-wide barrier is in the loop, and the copies run on
-//     across items;
+//   - a block's four warps take 16 positions at a time each.  A warp (a team of 2 or 4 warps where G > 16: one for each
+//     16 heads) has a ring of its own in shared memory, filled by 16-byte asynchronous copies that gather rows by the
+//     table, whose entries come into shared memory several steps before.  No block-wide barrier is in the loop, and the
+//     copies run on across items;
 //   - the products are m16n8k16 matrix instructions with the 16 heads as rows: scores and probabilities stay in
-//     registers (the scores' layout is the layout that the second product wants), the softmax's running maximum and
-//     sum in 32 bits; the output accumulates in registers and is rescaled only where a maximum moved;
-//   - where an item is cut, each block leaves its maximum, sum and output in the workspace and the second kernel joins
-//     them in the order of the positions (the same bits each time).  It is launched early (programmatic dependent
-//     launch) and waits for the first.  It also turns the scores, left in the workspace in 32 bits, into weights: their
-//     sum over the group needs each head's final lse, and reading 4 * G bytes back costs less than the key again.
+//     registers (the scores' layout is the layout that the second product wants), with the softmax's running maximum and
+//     sum in 32 bits; the output accumulates in registers.  Tensor memory would put a key in each of its 128 lanes and so
+//     each maximum over keys across lanes, for a product that takes 6% of the tensor cores;
+//   - where an item is cut, each block leaves its maximum, sum and output in the workspace and a second kernel joins them
+//     in the order of the positions (the same bits each time).  It also turns the scores, left in the workspace in 32
+//     bits, into weights: their sum over the group needs each head's final lse, and reading 4 * G bytes back costs less
+//     than the key again;
+//   - work so short that the second kernel would be a third of the time goes to clusters instead: one for each item, of
+//     blocks with eight warps, which join their item through distributed shared memory.
+// Measured (main kernel and join; a plain streaming read of the same bytes in brackets): 131072 positions of 2 x 128,
+// G = 16: 25.3 + 6.8 us (24.8); 64 sequences of 4096 to 65536, 2.28 GB: 349 + 4.9 us, 6.5 TB/s (347); table entries
+// read one step ahead only, 381 + 4.8; G = 32 over 134 MB 27.5 + 5.4, G = 64 43.6 + 8.7, where the matrix instructions'
+// and the softmax's latency shows.
 // Roundings: the probabilities go to the cache's type for the product with v (the sum l uses them unrounded), and the
 // output once at the end.
 #include <cuda_bf16.h>
@@ -36,7 +43,7 @@
 namespace {
 
 constexpr int kBlocksPerSm = 2;
-constexpr int kGrain = 2;            // units a block takes at least: below it the join costs more than the split gains
+constexpr int kGrain = 2;            // units a block takes at least (1, 2 and 4 differ by less than 0.5 us)
 constexpr int kMaxWorkers = 296;     // resident blocks, at most: two on each of 148 SMs
 constexpr uint32_t kRingBytes = 96 * 1024;      // two blocks an SM
 constexpr uint32_t kNearRingBytes = 192 * 1024;  // one: clusters that join their items have SMs to themselves
@@ -44,9 +51,13 @@ constexpr int kMaxG = 64;
 constexpr int kMaxDevices = 64;
 constexpr int kMaxUnit = 256;
 constexpr int kMaxCluster = 16;
-constexpr int kNearWork = 1024 * 128;  // positions times head dim of a cluster's block, at most
+// Positions times head dim of a cluster's block, at most: where the clusters fill half of the SMs, and where they do not
+// and dealing out would use the others.  Measured, cluster against dealt out and joined: one sequence of 217 positions
+// 6.9 / 8.8 us, 1000 7.3 / 9.0, 4000 9.3 / 10.3, 8192 11.1 / 9.9; 64 of up to 500 10.8 / 13.9, 32 of up to 2000
+// 14.3 / 17.3, 7 of up to 2501 with 8 kv heads of 64 9.6 / 11.2.
+constexpr int kNearWork = 1024 * 128, kNearWorkAlone = 384 * 128;
 constexpr int kJoinThreads = 512;
-constexpr float kLag = 6.f;
+constexpr float kLag = 6.f;          // of the maximum taken out, see there; 0 costs 0.3 of 9.6 us for 7 sequences of up to 2501
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -978,7 +989,7 @@ template <typename T, int D, int MT> int launch(const Params &p, cudaStream_t s)
             ++i;
         const int64_t C = 1 << i;
         if (items <= active_clusters((const void *)kernel, cfg, known, i) &&
-            (units + C - 1) / C * S::kUnit * D <= kNearWork) {
+            (units + C - 1) / C * S::kUnit * D <= (2 * items * C >= unum::sm_count() ? kNearWork : kNearWorkAlone)) {
             cfg.gridDim = dim3((unsigned)(items * C));
             attr[0].val.clusterDim.x = (unsigned)C;
             cfg.numAttrs = 2;
