@@ -603,7 +603,22 @@ __global__ void __launch_bounds__(Shape<D, MT, kNear>::kThreads, kNear ? 1 : kBl
                 float s[kStep / 8][4];
 #pragma unroll
                 for (int t = 0; t < kStep / 8; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
-                if (mask) {
+                if (kStep == 16 && mask) {
+                    // two chains of products for each 8 positions: half the latency, half the roundings in a row
+                    float e[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; kk += 2) {
+                        uint32_t f[4], g[4];
+                        ldsm4(f, kb ^ (kk << 5));
+                        ldsm4(g, kb ^ ((kk + 1) << 5));
+                        Num<T>::mma(s[0], qa[kk], f[0], f[1]);
+                        Num<T>::mma(s[1], qa[kk], f[2], f[3]);
+                        Num<T>::mma(e[0], qa[kk + 1], g[0], g[1]);
+                        Num<T>::mma(e[1], qa[kk + 1], g[2], g[3]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] += e[i >> 2][i & 3];
+                } else if (mask) {
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
