@@ -135,6 +135,7 @@ __device__ __forceinline__ int32_t cluster_rank() {
     return r;
 }
 __device__ __forceinline__ void cluster_arrive() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -411,7 +412,6 @@ __device__ __forceinline__ void join_cluster(const Params &p, const float (&o)[D
         j.add(C, [&](int r, float2 &a, float2 &, float4 &) { a = ld_cluster2(peer(&ml[tid], r)); });
         z[tid] = lse2_of(j.ml0);
     }
-    __syncwarp();
     cluster_arrive();
     if (p.weights) {
         __syncthreads();

@@ -102,6 +102,7 @@ __device__ __forceinline__ uint32_t cluster_size() {
 }
 
 __device__ __forceinline__ void cluster_arrive() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
 
