@@ -70,7 +70,7 @@ constexpr int kMaxCluster = 16;
 constexpr int64_t kMaxSlice = 25600;  // 4 bytes a page: 100 KB of shared memory
 constexpr int64_t kMaxPages = kMaxCluster * kMaxSlice;
 constexpr int kBins = 256;
-constexpr int kGroups = kEvThreads / kBins;
+constexpr int kGroups = 2 * kEvThreads / kBins;
 constexpr int kCopies = 8;   // of the histogram
 constexpr int kBatch = 4;    // loads of a thread under way
 
@@ -140,8 +140,9 @@ __device__ __forceinline__ uint32_t scan_warps(uint32_t v, uint32_t *warp_sums, 
 // kVec: pages of 4 positions and more whose weights 16-byte loads can read.
 template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kernel(const __grid_constant__ EvictParams p) {
     extern __shared__ uint32_t keys[];  // this block's slice
-    __shared__ uint32_t hist[kCopies][kBins], counts[4][kBins];  // counts: this block's, of each digit
-    __shared__ uint32_t sums[kGroups][kBins];                    // the cluster's, of every kGroups-th block
+    __shared__ __align__(8) uint32_t hist[kCopies][kBins];
+    __shared__ uint32_t counts[4][kBins / 2];             // this block's, of each digit
+    __shared__ __align__(8) uint32_t sums[kGroups][kBins];  // the cluster's, of every kGroups-th block
     __shared__ uint32_t warp_sums[kEvWarps];
     __shared__ uint32_t found[3];    // the digit, how many are still wanted with it, and how many have it
     __shared__ uint32_t slice_eq, slice_sure;
@@ -264,22 +265,28 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
                 }
             }
             __syncthreads();
-            if (tid < kBins) {
+            if (tid < kBins / 2) {  // two counts a word: a slice has fewer pages than 2^16
                 uint32_t c = 0;
 #pragma unroll
                 for (int i = 0; i < kCopies; ++i) {
-                    c += hist[i][tid];
-                    hist[i][tid] = 0;
+                    const uint2 h = *reinterpret_cast<uint2 *>(&hist[i][2 * tid]);
+                    c += h.x | h.y << 16;
+                    *reinterpret_cast<uint2 *>(&hist[i][2 * tid]) = make_uint2(0, 0);
                 }
                 counts[d][tid] = c;
             }
             if (C > 1) cluster_barrier();
             else __syncthreads();
             {
-                uint32_t c = 0;
-#pragma unroll 8
-                for (uint32_t r = tid / kBins; r < C; r += kGroups) c += C > 1 ? ld_cluster(peer(&counts[d][tid % kBins], r)) : counts[d][tid % kBins];
-                sums[tid / kBins][tid % kBins] = c;
+                const int pair = tid % (kBins / 2), group = tid / (kBins / 2);
+                uint32_t c0 = 0, c1 = 0;
+#pragma unroll 4
+                for (uint32_t r = group; r < C; r += kGroups) {
+                    const uint32_t c = C > 1 ? ld_cluster(peer(&counts[d][pair], r)) : counts[d][pair];
+                    c0 += c & 0xffffu;
+                    c1 += c >> 16;
+                }
+                *reinterpret_cast<uint2 *>(&sums[group][2 * pair]) = make_uint2(c0, c1);
             }
             __syncthreads();
             if (warp == 0) {  // lane l has digits 255 - 8l .. 248 - 8l: a scan from the top
