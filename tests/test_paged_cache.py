@@ -517,6 +517,46 @@ def test_calls_behind_kernels_that_still_run(lens):
         assert all(torch.equal(a, b) for a, b in zip(got[4], paged_attention(q, kc3, vc3, table, ln, return_lse=True)))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[900, 20, 300], [30000, 20, 17000]])
+def test_calls_on_several_streams_at_once(lens):
+    """Calls that overlap have workspaces of their own."""
+    from unum_ops_b200 import paged_attention
+
+    q, kc, vc, table, ln = [x.to(dev()) for x in make_case(3, lens, 2, 16, 128, 1, "bf16")]
+    qs = [q * (i + 1) / 3 for i in range(4)]
+    want = [paged_attention(x, kc, vc, table, ln, return_lse=True) for x in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    for _ in range(20):
+        got = []
+        for s, x in zip(streams, qs):
+            with torch.cuda.stream(s):
+                got.append(paged_attention(x, kc, vc, table, ln, return_lse=True))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+
+@pytest.mark.gpu
+def test_large_batches():
+    """More sequences than there are threads in a block, or blocks on the GPU."""
+    from unum_ops_b200 import evict_cache
+
+    rng = np.random.default_rng(8)
+    for B, longest, Hk, G in ((6000, 40, 1, 4), (1500, 300, 2, 16), (70000, 3, 1, 1)):
+        lens = rng.integers(0, longest + 1, B)
+        q, kc, vc, table, _ = make_case(7, np.maximum(lens, 1), Hk, G, 64, 1, "bf16")
+        ln = torch.from_numpy(lens.astype(np.int32))
+        before = torch.from_numpy(rng.random((B, Hk, table.shape[1])).astype(np.float32))
+        out, lse, after = run_attention(q, kc, vc, table, ln, 1, before)
+        check_attention(q, kc, vc, table, ln, 1, 64 ** -0.5, out, lse, before, after)
+    lens, w = rng.integers(0, 201, 2000).astype(np.int32), rng.random((2000, 2, 200)).astype(np.float32)
+    table = np.arange(2000 * 200, dtype=np.int32).reshape(2000, 200)
+    got = evict_cache(*[torch.from_numpy(x).to(dev()) for x in (table, lens, w)], budget=64, local_pages=3)
+    for x, y in zip(got, oracle_evict(table, lens, w, 64, 0, 3, 1)):
+        np.testing.assert_array_equal(x.cpu().numpy(), y)
+
+
 # ------------------------------------------------------------------------------------------------ append (GPU)
 @pytest.mark.gpu
 @pytest.mark.parametrize("T,B,Hk,D,page,dtype", [(1, 1, 2, 128, 1, "bf16"), (7, 3, 1, 64, 4, "fp16"), (500, 5, 8, 64, 16, "bf16"),
