@@ -62,6 +62,8 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
 //            blocks: they are served one at a time.)
 //   write    each warp has a contiguous part of the slice; a count and one scan over the warps give each page its
 //            place, among those that stay or among the evicted, and the weights move along.
+// Where the first and the last pages fill the budget nothing is chosen: places go by the index alone, and no key is made
+// or read.
 // What is filled behind the new ends does not wait for any of it and is written first.
 // Bound by latency for one sequence (the barriers), by HBM for a batch.
 constexpr int kEvThreads = 512;  // with 1024, block barriers cost more than the added warps hid (12.5 against 10.3 us)
@@ -154,6 +156,8 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
     len = len < 0 ? 0 : (len > p.n_pages * P ? p.n_pages * P : len);
     const int64_t used = (len + P - 1) >> p.shift;
     const int64_t drop = used > p.budget ? used - p.budget : 0;
+    uint32_t want = (uint32_t)(p.budget - p.init - p.local);  // pages that stay by their weight
+    const bool chosen = drop > 0 && want > 0;                 // and only then are there keys
     const int64_t per = (used + C - 1) / C;
     const int64_t s0 = per * rank < used ? per * rank : used;
     const int64_t s1 = s0 + per < used ? s0 + per : used;
@@ -173,7 +177,7 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
     int64_t kept_before = s0;
     uint32_t stay_at = i0;
     // keys from edge_from on stay; of those equal to edge, eq_left (eq_at: so far)
-    uint32_t edge = 0, edge_from = 0, eq_at = 0, eq_left = 0;
+    uint32_t edge = 0xffffffffu, edge_from = 0xffffffffu, eq_at = 0, eq_left = 0;  // no key is that large
 
     // behind what stays: pages of the row that are not in use yet move up, and nothing fills the rest
     const int64_t me = (int64_t)rank * kEvThreads + tid, all_threads = (int64_t)C * kEvThreads;
@@ -194,7 +198,7 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
             for (int64_t j = end + me; j < p.W; j += all_threads) nwb[h * p.W + j] = 0.0f;
     }
 
-    if (drop > 0) {
+    if (chosen) {
         for (int i = tid; i < kCopies * kBins; i += kEvThreads) (&hist[0][0])[i] = 0;
         __syncthreads();
         // keys; `lanes` threads share a page
@@ -251,11 +255,9 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
             }
         }
         // the key of the lightest page that stays, digit by digit
-        uint32_t prefix = 0, all_from = 0xffffffffu;  // no key is that large
-        uint32_t want = (uint32_t)(p.budget - p.init - p.local);  // candidates that stay
-        const bool any = want > 0;
+        uint32_t prefix = 0, all_from = 0;
         my_hist = hist[lane & (kCopies - 1)];
-        for (int d = 0; d < 4 && any; ++d) {
+        for (int d = 0; d < 4; ++d) {
             const int sh = 24 - 8 * d;
             if (d > 0) {
 #pragma unroll 4
@@ -325,15 +327,18 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
             }
             if (d == 3) ++all_from;
         }
-        if (!any) prefix = 0xffffffffu;
-        // Keys from all_from on stay, and of the pages with the key `prefix` the first `want`.  What this warp's part has
+        edge = prefix;
+        edge_from = all_from;
+    }
+    if (drop > 0) {
+        // Keys from edge_from on stay, and of the pages with the key `edge` the first `want`.  What this warp's part has
         // of either:
         uint32_t n_sure = 0, n_eq = 0;
         for (int32_t i = i0 + lane; i < i1; i += 32) {
-            const uint32_t key = keys[i];
-            const bool s = i < cand0 || i >= cand1 || key >= all_from;
+            const uint32_t key = chosen ? keys[i] : 0;
+            const bool s = i < cand0 || i >= cand1 || key >= edge_from;
             n_sure += s;
-            n_eq += !s && key == prefix;
+            n_eq += !s && key == edge;
         }
         n_sure = __reduce_add_sync(0xffffffffu, n_sure);
         n_eq = __reduce_add_sync(0xffffffffu, n_eq);
@@ -352,12 +357,9 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
             sure_before += ld_cluster(peer(&slice_sure, r));
         }
         if (C > 1) cluster_arrive();  // waited for at the end: no block leaves while another reads its shared memory
-        if (!any) want = 0;
         eq_left = want - min(eq_before, want);  // of this slice's, the first ones
         kept_before = sure_before + min(eq_before, want);
         stay_at = sure_at + min(eq_at, eq_left);
-        edge = prefix;
-        edge_from = all_from;
     }
     // places.  The warp's list of pages that stay takes the room of its keys, behind where it reads.
     const int64_t to = (kept_before + stay_at) << p.shift;
@@ -369,7 +371,7 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
         const uint32_t below = (1u << lane) - 1;
         bool stay = i < i1;
         if (drop > 0) {
-            const uint32_t key = stay ? keys[i] : 0;
+            const uint32_t key = stay && chosen ? keys[i] : 0;
             const bool sure = stay && (i < cand0 || i >= cand1 || key >= edge_from);
             const bool eq = stay && !sure && key == edge;
             const uint32_t eqs = __ballot_sync(0xffffffffu, eq);
