@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_paged_cache import dev, make_case, oracle_evict
+from test_paged_cache import DT, dev, make_case, np64, oracle_evict
 
 
 # ------------------------------------------------------------------------------------------------ eviction
@@ -36,3 +36,65 @@ def test_eviction_to_the_first_and_last_pages(lens, page, init, local):
         got = evict_cache(*args, budget=init + local, init_pages=init, local_pages=local, page_size=page)
         for name, x, y in zip(("table", "seqlens", "weights", "evicted"), got, want):
             np.testing.assert_array_equal(x.cpu().numpy(), y, err_msg=name)
+
+
+# ------------------------------------------------------------------------------------------------ values that few bits lose
+# The kernels hold a probability in the cache's type as 2^(s - m + lift), m a maximum of the scores (base 2) of the warp's
+# positions and lift 12 in fp16.  A rounding is off by eps/2 of the probability, or where that is subnormal by half of the
+# smallest subnormal: 2^-25 in fp16, 2^-37 of the largest probability.  The sum of all is at least the largest, so
+#     |err| <= eps/2 * (|out| + sum p|v|) + 2^-16 * sum p|v| + 2^-37 * sum |v| + 2^-25 (fp16's subnormal outputs)
+# with the scores exact here (one product each).  In bf16, whose exponents are fp32's, the last two are 0.
+@pytest.mark.gpu
+@pytest.mark.parametrize("gap", [0, 10, 14, 17, 18, 24])
+@pytest.mark.parametrize("n,Hk,G,D,at,spread", [(16, 1, 1, 64, 0, 0), (700, 2, 16, 128, 0, 1), (16384, 1, 16, 128, 0, 0), (16384, 2, 4, 64, 9000, 1),
+                                                (40000, 2, 16, 128, 39999, 1), (9000, 1, 33, 64, 4, 0), (131072, 1, 16, 128, 0, 1)])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_one_key_far_above_the_others(dtype, n, Hk, G, D, at, spread, gap):
+    """An attention sink: one key `gap` nats above the others' mean, its value 0.  The others are the output."""
+    from unum_ops_b200 import paged_attention
+
+    rng = np.random.default_rng(n + G)
+    t = lambda x: torch.from_numpy(x.astype(np.float32)).to(DT[dtype])  # noqa: E731
+    q, k = np.zeros((1, Hk * G, D)), np.zeros((n, Hk, D))
+    q[:, :, 0], k[:, :, 0] = 1, spread * rng.standard_normal((n, Hk))
+    k[at, :, 0] = gap
+    v = rng.uniform(0.5, 8, (n, Hk, D))
+    v[at] = 0
+    q, k, v = t(q), t(k), t(v)
+    d = dev()
+    out = np64(paged_attention(q.to(d), k.to(d), v.to(d), torch.arange(n, dtype=torch.int32, device=d)[None],
+                               torch.tensor([n], dtype=torch.int32, device=d), softmax_scale=1.0))[0].reshape(Hk, G, D)
+    s = np64(k)[:, :, 0]
+    p = np.exp(s - s.max(0))
+    p /= p.sum(0)
+    ref = np.einsum("nh,nhd->hd", p, np64(v))[:, None]  # the values are positive: sum p|v| as well
+    small = 2.0 ** -37 * np64(v).sum(0)[:, None] + 2.0 ** -25 if dtype == "fp16" else 0
+    allow = 2 * torch.finfo(DT[dtype]).eps / 2 * ref + 2.0 ** -16 * ref + small
+    err = np.abs(out - ref)
+    assert np.all(err <= allow), f"off by {np.max(err / allow)} of what is allowed"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,G", [(1000, 16), (1000, 32), (40000, 16)])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_scores_of_any_magnitude(dtype, n, G):
+    """Scores from 1 to 2^31, a few of their last places apart: their maximum is taken out without what it is shifted by
+    being rounded into an overflow.  All values are 1, and so is the output, to a rounding of each probability and one of
+    the output."""
+    from unum_ops_b200 import paged_attention
+
+    d = dev()
+    rng = np.random.default_rng(n)
+    heads = 2 * G
+    q, k = torch.zeros(1, heads, 64), torch.zeros(n, 2, 64)
+    q[..., 0] = 32768.0
+    q[..., 1] = torch.from_numpy(np.exp2(rng.integers(0, 8, heads)))
+    k[..., 1] = torch.from_numpy(rng.uniform(0, 30, (n, 2)))
+    v = torch.ones(n, 2, 64, dtype=DT[dtype], device=d)
+    table, ln = torch.arange(n, dtype=torch.int32, device=d)[None], torch.tensor([n], dtype=torch.int32, device=d)
+    for e in range(-15, 16):
+        for sign in (1, -1):
+            k[..., 0] = sign * 2.0 ** e * torch.from_numpy(rng.uniform(1, 1.001 if e < 4 else 1, (n, 2)))
+            out = paged_attention(q.to(DT[dtype]).to(d), k.to(DT[dtype]).to(d), v, table, ln, softmax_scale=1.0).double()
+            err = float((out - 1).abs().nan_to_num(nan=float("inf")).max())
+            assert err <= torch.finfo(DT[dtype]).eps + 2.0 ** -16, (e, sign, err)

@@ -32,7 +32,8 @@
 // read one step ahead only, 381 + 4.8; G = 32 over 134 MB 27.5 + 5.4, G = 64 43.6 + 8.7, where the matrix instructions'
 // and the softmax's latency shows.
 // Roundings: the probabilities go to the cache's type for the product with v (the sum l uses them unrounded), and the
-// output once at the end.
+// output once at the end.  The matrix instructions take no wider type beside the cache's; of an output's error against 64
+// bits, 1.7e-3 of its norm in bf16 and 2.1e-4 in fp16 with the last rounding alone, the two make 2.4e-3 and 2.7e-4.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -57,7 +58,6 @@ constexpr int kMaxCluster = 16;
 // 14.3 / 17.3, 7 of up to 2501 with 8 kv heads of 64 9.6 / 11.2.
 constexpr int kNearWork = 1024 * 128, kNearWorkAlone = 384 * 128;
 constexpr int kJoinThreads = 512;
-constexpr float kLag = 6.f;          // of the maximum taken out, see there; 0 costs 0.3 of 9.6 us for 7 sequences of up to 2501
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -167,8 +167,10 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// kLift, kLag: see where the maximum is taken out
 template <typename T> struct Num;
 template <> struct Num<__nv_bfloat16> {
+    static constexpr float kLift = 0.f, kUnlift = 1.f, kLag = 6.f;
     static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                      "{%0, %1, %2, %3};"
@@ -181,6 +183,7 @@ template <> struct Num<__nv_bfloat16> {
     }
 };
 template <> struct Num<__half> {
+    static constexpr float kLift = 12.f, kUnlift = 1.f / 4096, kLag = 3.f;  // kUnlift = 2^-kLift
     static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                      "{%0, %1, %2, %3};"
@@ -346,7 +349,10 @@ struct Joined {
     }
 };
 
-__device__ __forceinline__ float lse2_of(float2 ml) { return ml.y != 0.f ? ml.x + log2f(ml.y) : -INFINITY; }
+// What was taken out lies kLift below a maximum: back to it first, so that the two do not cancel.
+template <typename T> __device__ __forceinline__ float lse2_of(float2 ml) {
+    return ml.y != 0.f ? ml.x + Num<T>::kLift + log2f(ml.y * Num<T>::kUnlift) : -INFINITY;
+}
 
 // The end of an item that a cluster has: the block's warps leave their outputs, maxima and sums (ml: of rows r0 and
 // r0 + 8) in shared memory and join them, tile by tile (8 columns of 16 heads); then each block joins some tiles of all
@@ -403,14 +409,14 @@ __device__ __forceinline__ void join_cluster(const Params &p, const float (&o)[D
         if (r0 + 8 < left) op[4 * D] = Num<T>::pack(j.o.z * i1, j.o.w * i1);
         if (p.lse && tile == 0 && (lane & 3) == 0) {
             float *l = p.lse + item * p.G + ht * 16 + r0;
-            if (r0 < left) l[0] = lse2_of(j.ml0) * kLn2;
-            if (r0 + 8 < left) l[8] = lse2_of(j.ml1) * kLn2;
+            if (r0 < left) l[0] = lse2_of<T>(j.ml0) * kLn2;
+            if (r0 + 8 < left) l[8] = lse2_of<T>(j.ml1) * kLn2;
         }
     }
     if (p.weights && tid < 16 * MT) {
         Joined j;
         j.add(C, [&](int r, float2 &a, float2 &, float4 &) { a = ld_cluster2(peer(&ml[tid], r)); });
-        z[tid] = lse2_of(j.ml0);
+        z[tid] = lse2_of<T>(j.ml0);
     }
     cluster_arrive();
     if (p.weights) {
@@ -433,6 +439,7 @@ template <typename T, int D, int MT, bool kNear>
 __global__ void __launch_bounds__(Shape<D, MT, kNear>::kThreads, kNear ? 1 : kBlocksPerSm)
     attend_kernel(const __grid_constant__ Params p) {
     using S = Shape<D, MT, kNear>;
+    using N = Num<T>;
     constexpr int kWarps = S::kWarps, kThreads = S::kThreads;
     constexpr int kTeams = S::kTeams, kStep = S::kStep, kSlots = S::kSlots, kRow = S::kRow, kUnit = S::kUnit;
     constexpr uint32_t kHalf = S::kHalf, kSlot = S::kSlot;
@@ -665,11 +672,15 @@ __global__ void __launch_bounds__(Shape<D, MT, kNear>::kThreads, kNear ? 1 : kBl
                     x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, i));
                     x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, i));
                 }
-                // The maximum taken out may stay behind the true one by up to 2^kLag: probabilities up to that are held as
-                // well, and the output is rescaled that much more rarely.
-                if (__any_sync(0xffffffffu, x0 > m0 + kLag || x1 > m1 + kLag)) {
-                    x0 = fmaxf(x0, m0);
-                    x1 = fmaxf(x1, m1);
+                // What is taken out lies kLift below a maximum, so that probabilities come to 2^kLift: fp16 has all its
+                // bits from 2^-14 on only, and would lose those of keys far below one that outshines them.  And the maximum
+                // may stay behind the true one by up to kLag: the output is rescaled that much more rarely.  Together they
+                // leave probabilities up to 2^15 in fp16, whose largest is just below 2^16.  The difference is what is
+                // looked at, and a maximum so large that its last place passes kLift is taken out as it is: neither limit
+                // holds after rounding otherwise.
+                if (__any_sync(0xffffffffu, x0 - m0 > N::kLift + N::kLag || x1 - m1 > N::kLift + N::kLag)) {
+                    x0 = fmaxf(x0 - (x0 - N::kLift) <= N::kLift ? x0 - N::kLift : x0, m0);
+                    x1 = fmaxf(x1 - (x1 - N::kLift) <= N::kLift ? x1 - N::kLift : x1, m1);
                     const float a0 = x0 == -INFINITY ? 1.f : ex2(m0 - x0), a1 = x1 == -INFINITY ? 1.f : ex2(m1 - x1);
                     m0 = x0;
                     m1 = x1;
@@ -782,7 +793,7 @@ __global__ void __launch_bounds__(Shape<D, MT, kNear>::kThreads, kNear ? 1 : kBl
         if (team == 0) {
             if (from_start && to_end) {  // the whole item
                 const float i0 = l0 != 0.f ? 1.f / l0 : 0.f, i1 = l1 != 0.f ? 1.f / l1 : 0.f;
-                const float z0 = l0 != 0.f ? m0 + log2f(l0) : -INFINITY, z1 = l1 != 0.f ? m1 + log2f(l1) : -INFINITY;
+                const float z0 = lse2_of<T>(make_float2(m0, l0)), z1 = lse2_of<T>(make_float2(m1, l1));
                 const int left = p.G - ht * 16;
                 uint32_t *op = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p.out) +
                                                             ((item * p.G + ht * 16 + r0) * D + c0) * 2);
@@ -865,7 +876,7 @@ __global__ void __launch_bounds__(kJoinThreads, 2) join_kernel(const __grid_cons
         for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
         const float inv = L != 0.f ? 1.f / L : 0.f;
         for (int32_t i = lane; i < parts; i += 32) ml[i][warp].x *= inv;
-        const float lse2 = L != 0.f ? M + log2f(L) : -INFINITY;
+        const float lse2 = lse2_of<T>(make_float2(M, L));
         if (lane == 0) z[ht * 16 + warp] = lse2;
         __syncthreads();
         return lse2;
