@@ -3,10 +3,14 @@ follow each other without a pause, ids of 64 bits, caches that share memory.
 
 The oracles are those of test_paged_cache.py: the operators' definition in 64 bits, position by position.
 """
+import os
+import re
+
 import numpy as np
 import pytest
 import torch
 
+from conftest import ROOT
 from test_paged_cache import DT, dev, make_case, np64, oracle_evict
 
 
@@ -98,3 +102,20 @@ def test_scores_of_any_magnitude(dtype, n, G):
             out = paged_attention(q.to(DT[dtype]).to(d), k.to(DT[dtype]).to(d), v, table, ln, softmax_scale=1.0).double()
             err = float((out - 1).abs().nan_to_num(nan=float("inf")).max())
             assert err <= torch.finfo(DT[dtype]).eps + 2.0 ** -16, (e, sign, err)
+
+
+# ------------------------------------------------------------------------------------------------ barriers
+def test_warps_come_together_before_the_barriers_that_ask_for_it():
+    """A cluster's barrier (.aligned) and bar.sync are for whole warps: in the paged cache's kernels and in what they share
+    with others, a __syncwarp stands before each."""
+    csrc, found = os.path.join(ROOT, "unum_ops_b200", "csrc"), 0
+    for name in ("paged_attention.cu", "paged_cache.cu", "sm100.cuh"):
+        with open(os.path.join(csrc, name)) as f:
+            text = re.sub(r"//[^\n]*", "", f.read())
+        for m in re.finditer(r"(if \([^)]*\)\s*|else\s*)?asm volatile\(\s*\"(barrier\.cluster\.\w+|bar\.sync)", text):
+            if name == "sm100.cuh" and m.group(2) == "bar.sync":
+                continue  # its callers' business: no paged kernel is one
+            found += 1
+            assert text[:m.start()].rstrip().endswith("__syncwarp();"), (name, m.group(0))
+        assert not re.search(r"\.aligned;\\n\\t *barrier", text), name
+    assert found >= 3

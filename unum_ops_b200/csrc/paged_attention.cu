@@ -40,8 +40,11 @@
 #include <atomic>
 
 #include "common.cuh"
+#include "sm100.cuh"
 
 namespace {
+
+using namespace unum::sm100;
 
 constexpr int kBlocksPerSm = 2;
 constexpr int kGrain = 2;            // units a block takes at least (1, 2 and 4 differ by less than 0.5 us)
@@ -82,8 +85,6 @@ struct Params {
 };
 
 // ---------------------------------------------------------------------------------------------- instructions
-__device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-
 __device__ __forceinline__ uint64_t evict_first() {
     uint64_t policy;
     asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
@@ -122,43 +123,6 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
 __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
-}
-
-__device__ __forceinline__ int32_t cluster_size() {
-    int32_t r;
-    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ int32_t cluster_rank() {
-    int32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_arrive() {
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_barrier() {
-    cluster_arrive();
-    cluster_wait();
-}
-// The address of this block's shared memory location in block `rank` of the cluster.
-__device__ __forceinline__ uint32_t peer(const void *mine, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(mine)), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ float2 ld_cluster2(uint32_t a) {
-    float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
-    return v;
-}
-__device__ __forceinline__ float4 ld_cluster4(uint32_t a) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
-    return v;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -391,15 +355,15 @@ __device__ __forceinline__ void join_cluster(const Params &p, const float (&o)[D
             ml[ht * 16 + r0 + 8] = j.ml1;
         }
     }
-    cluster_barrier();
+    cluster_sync();
 #pragma unroll 1
     for (int t = warp * C + rank; t < MT * kTiles; t += kWarps * C) {
         const int ht = t / kTiles, tile = t - ht * kTiles;
         Joined j;
         j.add(C, [&](int r, float2 &a, float2 &b, float4 &v) {
-            a = ld_cluster2(peer(&ml[ht * 16 + r0], r));
-            b = ld_cluster2(peer(&ml[ht * 16 + r0 + 8], r));
-            v = ld_cluster4(peer(&box[t * 32 + lane], r));
+            a = ld_cluster_f32x2(peer_smem(&ml[ht * 16 + r0], r));
+            b = ld_cluster_f32x2(peer_smem(&ml[ht * 16 + r0 + 8], r));
+            v = ld_cluster_f32x4(peer_smem(&box[t * 32 + lane], r));
         });
         const float i0 = j.ml0.y != 0.f ? 1.f / j.ml0.y : 0.f, i1 = j.ml1.y != 0.f ? 1.f / j.ml1.y : 0.f;
         const int left = p.G - ht * 16;
@@ -415,7 +379,7 @@ __device__ __forceinline__ void join_cluster(const Params &p, const float (&o)[D
     }
     if (p.weights && tid < 16 * MT) {
         Joined j;
-        j.add(C, [&](int r, float2 &a, float2 &, float4 &) { a = ld_cluster2(peer(&ml[tid], r)); });
+        j.add(C, [&](int r, float2 &a, float2 &, float4 &) { a = ld_cluster_f32x2(peer_smem(&ml[tid], r)); });
         z[tid] = lse2_of<T>(j.ml0);
     }
     cluster_arrive();
@@ -430,8 +394,8 @@ __device__ __forceinline__ void join_cluster(const Params &p, const float (&o)[D
 }
 
 template <int MT> __device__ __forceinline__ void team_sync(int team) {
-    if (MT == 1) __syncwarp();
-    else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(MT * 32) : "memory");
+    __syncwarp();  // the barrier too is one that whole warps execute together
+    if (MT > 1) asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(MT * 32) : "memory");
 }
 
 // kNear: a cluster has one item and joins it itself.
@@ -458,7 +422,7 @@ __global__ void __launch_bounds__(Shape<D, MT, kNear>::kThreads, kNear ? 1 : kBl
 
     // Launched while the kernel before it may still run, and lets the one behind it do so.
     unum::wait_for_previous_kernel();
-    const int32_t C = kNear ? cluster_size() : 1, rank = kNear ? cluster_rank() : 0, me = blockIdx.x;
+    const int32_t C = kNear ? cluster_nctarank() : 1, rank = kNear ? cluster_ctarank() : 0, me = blockIdx.x;
     int32_t u0, u1;
     Place<kUnit> in;  // where the entries are read
     Shares shares;

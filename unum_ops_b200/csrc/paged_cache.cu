@@ -16,8 +16,11 @@
 #include <cuda_runtime.h>
 
 #include "common.cuh"
+#include "sm100.cuh"
 
 namespace {
+
+using namespace unum::sm100;
 
 // ------------------------------------------------------------------------------------------------ append
 // One thread moves the same 16 bytes of the key and of the value row.  The rows' loads do not wait for the
@@ -91,43 +94,6 @@ __device__ __forceinline__ uint32_t order_key(float x) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-
-__device__ __forceinline__ uint32_t cluster_size() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-
-__device__ __forceinline__ void cluster_arrive() {
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-
-__device__ __forceinline__ void cluster_barrier() {
-    cluster_arrive();
-    cluster_wait();
-}
-
-// The address of this block's shared memory location in block `rank` of the cluster.
-__device__ __forceinline__ uint32_t peer(const void *mine, uint32_t rank) {
-    uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(mine)), r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
-    return r;
-}
-
-__device__ __forceinline__ uint32_t ld_cluster(uint32_t a) {
-    uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-    return v;
-}
-
 // Exclusive scan over the block's warps of a value that each warp's lanes agree on, and the total.
 __device__ __forceinline__ uint32_t scan_warps(uint32_t v, uint32_t *warp_sums, uint32_t &total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -149,7 +115,7 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
     __shared__ uint32_t found[3];    // the digit, how many are still wanted with it, and how many have it
     __shared__ uint32_t slice_eq, slice_sure;
     unum::wait_for_previous_kernel();
-    const uint32_t rank = cluster_rank(), C = cluster_size();
+    const uint32_t rank = cluster_ctarank(), C = cluster_nctarank();
     const int64_t b = blockIdx.x / C;
     const int32_t P = 1 << p.shift;
     int64_t len = __ldg(p.seqlens + b);
@@ -277,14 +243,14 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
                 }
                 counts[d][tid] = c;
             }
-            if (C > 1) cluster_barrier();
+            if (C > 1) cluster_sync();
             else __syncthreads();
             {
                 const int pair = tid % (kBins / 2), group = tid / (kBins / 2);
                 uint32_t c0 = 0, c1 = 0;
 #pragma unroll 4
                 for (uint32_t r = group; r < C; r += kGroups) {
-                    const uint32_t c = C > 1 ? ld_cluster(peer(&counts[d][pair], r)) : counts[d][pair];
+                    const uint32_t c = C > 1 ? ld_cluster_u32(peer_smem(&counts[d][pair], r)) : counts[d][pair];
                     c0 += c & 0xffffu;
                     c1 += c >> 16;
                 }
@@ -349,12 +315,12 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
             slice_eq = all_eq;
             slice_sure = all_sure;
         }
-        if (C > 1) cluster_barrier();
+        if (C > 1) cluster_sync();
         // slices before this one: their pages of that key come first
         uint32_t eq_before = 0, sure_before = 0;
         for (uint32_t r = 0; r < rank; ++r) {
-            eq_before += ld_cluster(peer(&slice_eq, r));
-            sure_before += ld_cluster(peer(&slice_sure, r));
+            eq_before += ld_cluster_u32(peer_smem(&slice_eq, r));
+            sure_before += ld_cluster_u32(peer_smem(&slice_sure, r));
         }
         if (C > 1) cluster_arrive();  // waited for at the end: no block leaves while another reads its shared memory
         eq_left = want - min(eq_before, want);  // of this slice's, the first ones
