@@ -65,8 +65,7 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
 //            blocks: they are served one at a time.)
 //   write    each warp has a contiguous part of the slice; a count and one scan over the warps give each page its
 //            place, among those that stay or among the evicted, and the weights move along.
-// Where the first and the last pages fill the budget nothing is chosen: places go by the index alone, and no key is made
-// or read.
+// Where the first and the last pages fill the budget nothing is chosen: no sums are taken, and places go by the index alone.
 // What is filled behind the new ends does not wait for any of it and is written first.
 // Bound by latency for one sequence (the barriers), by HBM for a batch.
 constexpr int kEvThreads = 512;  // with 1024, block barriers cost more than the added warps hid (12.5 against 10.3 us)
@@ -122,8 +121,6 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
     len = len < 0 ? 0 : (len > p.n_pages * P ? p.n_pages * P : len);
     const int64_t used = (len + P - 1) >> p.shift;
     const int64_t drop = used > p.budget ? used - p.budget : 0;
-    uint32_t want = (uint32_t)(p.budget - p.init - p.local);  // pages that stay by their weight
-    const bool chosen = drop > 0 && want > 0;                 // and only then are there keys
     const int64_t per = (used + C - 1) / C;
     const int64_t s0 = per * rank < used ? per * rank : used;
     const int64_t s1 = s0 + per < used ? s0 + per : used;
@@ -143,7 +140,7 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
     int64_t kept_before = s0;
     uint32_t stay_at = i0;
     // keys from edge_from on stay; of those equal to edge, eq_left (eq_at: so far)
-    uint32_t edge = 0xffffffffu, edge_from = 0xffffffffu, eq_at = 0, eq_left = 0;  // no key is that large
+    uint32_t edge = 0, edge_from = 0, eq_at = 0, eq_left = 0;
 
     // behind what stays: pages of the row that are not in use yet move up, and nothing fills the rest
     const int64_t me = (int64_t)rank * kEvThreads + tid, all_threads = (int64_t)C * kEvThreads;
@@ -164,147 +161,149 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
             for (int64_t j = end + me; j < p.W; j += all_threads) nwb[h * p.W + j] = 0.0f;
     }
 
-    if (chosen) {
-        for (int i = tid; i < kCopies * kBins; i += kEvThreads) (&hist[0][0])[i] = 0;
-        __syncthreads();
-        // keys; `lanes` threads share a page
-        constexpr int kWide = kVec ? 4 : 1;
-        const int lanes = P < 32 * kWide ? P / kWide : 32;
-        const int sub = (tid & (lanes - 1)) * kWide;
-        const int32_t stride = kEvThreads / lanes;
-        uint32_t *my_hist = hist[lane & (kCopies - 1)];
-        if (lanes >= kCopies) my_hist = hist[(tid / lanes) & (kCopies - 1)];
-        for (int32_t i00 = tid / lanes; i00 < n + tid / lanes; i00 += kBatch * stride) {
-            double sum[kBatch] = {};
-            for (int32_t j = sub; j < P; j += lanes * kWide) {
-#pragma unroll 2
-                for (int32_t h = 0; h < p.Hk; ++h) {
-                    const float *src = wb + h * p.w_sh + (s0 << p.shift) + j;
-                    if (kVec) {
-                        float4 v[kBatch];
-#pragma unroll
-                        for (int e = 0; e < kBatch; ++e)
-                            if (i00 + e * stride < n)
-                                v[e] = __ldg(reinterpret_cast<const float4 *>(src + ((int64_t)(i00 + e * stride) << p.shift)));
-#pragma unroll
-                        for (int e = 0; e < kBatch; ++e) {
-                            const int64_t left = len - ((s0 + i00 + e * stride) << p.shift) - j;
-                            if (left >= 4) {
-                                sum[e] += ((double)v[e].x + (double)v[e].y) + ((double)v[e].z + (double)v[e].w);
-                            } else {
-                                if (left > 0) sum[e] += (double)v[e].x;
-                                if (left > 1) sum[e] += (double)v[e].y;
-                                if (left > 2) sum[e] += (double)v[e].z;
-                            }
-                        }
-                    } else {
-                        float v[kBatch];
-#pragma unroll
-                        for (int e = 0; e < kBatch; ++e) {
-                            const int64_t at = ((int64_t)(i00 + e * stride) << p.shift);
-                            v[e] = i00 + e * stride < n && (s0 << p.shift) + at + j < len ? __ldg(src + at) : 0.0f;
-                        }
-#pragma unroll
-                        for (int e = 0; e < kBatch; ++e) sum[e] += (double)v[e];
-                    }
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < kBatch; ++e) {
-                for (int o = lanes >> 1; o > 0; o >>= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], o);
-                const int32_t i = i00 + e * stride;
-                if (i < n && sub == 0) {
-                    const uint32_t key = order_key((float)sum[e]);
-                    keys[i] = key;
-                    if (i >= cand0 && i < cand1) atomicAdd(&my_hist[key >> 24], 1u);
-                }
-            }
-        }
-        // the key of the lightest page that stays, digit by digit
-        uint32_t prefix = 0, all_from = 0;
-        my_hist = hist[lane & (kCopies - 1)];
-        for (int d = 0; d < 4; ++d) {
-            const int sh = 24 - 8 * d;
-            if (d > 0) {
-#pragma unroll 4
-                for (int32_t i = cand0 + tid; i < cand1; i += kEvThreads) {
-                    const uint32_t key = keys[i];
-                    if ((key >> (sh + 8)) == prefix) atomicAdd(&my_hist[(key >> sh) & 255u], 1u);
-                }
-            }
-            __syncthreads();
-            if (tid < kBins / 2) {  // two counts a word: a slice has fewer pages than 2^16
-                uint32_t c = 0;
-#pragma unroll
-                for (int i = 0; i < kCopies; ++i) {
-                    const uint2 h = *reinterpret_cast<uint2 *>(&hist[i][2 * tid]);
-                    c += h.x | h.y << 16;
-                    *reinterpret_cast<uint2 *>(&hist[i][2 * tid]) = make_uint2(0, 0);
-                }
-                counts[d][tid] = c;
-            }
-            if (C > 1) cluster_sync();
-            else __syncthreads();
-            {
-                const int pair = tid % (kBins / 2), group = tid / (kBins / 2);
-                uint32_t c0 = 0, c1 = 0;
-#pragma unroll 4
-                for (uint32_t r = group; r < C; r += kGroups) {
-                    const uint32_t c = C > 1 ? ld_cluster_u32(peer_smem(&counts[d][pair], r)) : counts[d][pair];
-                    c0 += c & 0xffffu;
-                    c1 += c >> 16;
-                }
-                *reinterpret_cast<uint2 *>(&sums[group][2 * pair]) = make_uint2(c0, c1);
-            }
-            __syncthreads();
-            if (warp == 0) {  // lane l has digits 255 - 8l .. 248 - 8l: a scan from the top
-                uint32_t c[8], sum = 0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    c[e] = 0;
-#pragma unroll
-                    for (int i = 0; i < kGroups; ++i) c[e] += sums[i][255 - 8 * lane - e];
-                    sum += c[e];
-                }
-                uint32_t above = sum;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const uint32_t y = __shfl_up_sync(0xffffffffu, above, o);
-                    if (lane >= o) above += y;
-                }
-                above -= sum;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (above < want && want <= above + c[e]) {
-                        found[0] = 255 - 8 * lane - e;
-                        found[1] = want - above;
-                        found[2] = c[e];
-                    }
-                    above += c[e];
-                }
-            }
-            __syncthreads();
-            prefix = (prefix << 8) | found[0];
-            want = found[1];
-            all_from = prefix << sh;
-            if (found[2] == want) {  // all of them
-                prefix = 0xffffffffu;
-                break;
-            }
-            if (d == 3) ++all_from;
-        }
-        edge = prefix;
-        edge_from = all_from;
-    }
     if (drop > 0) {
-        // Keys from edge_from on stay, and of the pages with the key `edge` the first `want`.  What this warp's part has
+        uint32_t want = (uint32_t)(p.budget - p.init - p.local);  // pages that stay by their weight
+        uint32_t prefix = 0xffffffffu, all_from = 0xffffffffu;    // no key is that large
+        if (want > 0) {
+            for (int i = tid; i < kCopies * kBins; i += kEvThreads) (&hist[0][0])[i] = 0;
+            __syncthreads();
+            // keys; `lanes` threads share a page
+            constexpr int kWide = kVec ? 4 : 1;
+            const int lanes = P < 32 * kWide ? P / kWide : 32;
+            const int sub = (tid & (lanes - 1)) * kWide;
+            const int32_t stride = kEvThreads / lanes;
+            uint32_t *my_hist = hist[lane & (kCopies - 1)];
+            if (lanes >= kCopies) my_hist = hist[(tid / lanes) & (kCopies - 1)];
+            for (int32_t i00 = tid / lanes; i00 < n + tid / lanes; i00 += kBatch * stride) {
+                double sum[kBatch] = {};
+                for (int32_t j = sub; j < P; j += lanes * kWide) {
+    #pragma unroll 2
+                    for (int32_t h = 0; h < p.Hk; ++h) {
+                        const float *src = wb + h * p.w_sh + (s0 << p.shift) + j;
+                        if (kVec) {
+                            float4 v[kBatch];
+    #pragma unroll
+                            for (int e = 0; e < kBatch; ++e)
+                                if (i00 + e * stride < n)
+                                    v[e] = __ldg(reinterpret_cast<const float4 *>(src + ((int64_t)(i00 + e * stride) << p.shift)));
+    #pragma unroll
+                            for (int e = 0; e < kBatch; ++e) {
+                                const int64_t left = len - ((s0 + i00 + e * stride) << p.shift) - j;
+                                if (left >= 4) {
+                                    sum[e] += ((double)v[e].x + (double)v[e].y) + ((double)v[e].z + (double)v[e].w);
+                                } else {
+                                    if (left > 0) sum[e] += (double)v[e].x;
+                                    if (left > 1) sum[e] += (double)v[e].y;
+                                    if (left > 2) sum[e] += (double)v[e].z;
+                                }
+                            }
+                        } else {
+                            float v[kBatch];
+    #pragma unroll
+                            for (int e = 0; e < kBatch; ++e) {
+                                const int64_t at = ((int64_t)(i00 + e * stride) << p.shift);
+                                v[e] = i00 + e * stride < n && (s0 << p.shift) + at + j < len ? __ldg(src + at) : 0.0f;
+                            }
+    #pragma unroll
+                            for (int e = 0; e < kBatch; ++e) sum[e] += (double)v[e];
+                        }
+                    }
+                }
+    #pragma unroll
+                for (int e = 0; e < kBatch; ++e) {
+                    for (int o = lanes >> 1; o > 0; o >>= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], o);
+                    const int32_t i = i00 + e * stride;
+                    if (i < n && sub == 0) {
+                        const uint32_t key = order_key((float)sum[e]);
+                        keys[i] = key;
+                        if (i >= cand0 && i < cand1) atomicAdd(&my_hist[key >> 24], 1u);
+                    }
+                }
+            }
+            // the key of the lightest page that stays, digit by digit
+            prefix = 0;
+            my_hist = hist[lane & (kCopies - 1)];
+            for (int d = 0; d < 4; ++d) {
+                const int sh = 24 - 8 * d;
+                if (d > 0) {
+    #pragma unroll 4
+                    for (int32_t i = cand0 + tid; i < cand1; i += kEvThreads) {
+                        const uint32_t key = keys[i];
+                        if ((key >> (sh + 8)) == prefix) atomicAdd(&my_hist[(key >> sh) & 255u], 1u);
+                    }
+                }
+                __syncthreads();
+                if (tid < kBins / 2) {  // two counts a word: a slice has fewer pages than 2^16
+                    uint32_t c = 0;
+    #pragma unroll
+                    for (int i = 0; i < kCopies; ++i) {
+                        const uint2 h = *reinterpret_cast<uint2 *>(&hist[i][2 * tid]);
+                        c += h.x | h.y << 16;
+                        *reinterpret_cast<uint2 *>(&hist[i][2 * tid]) = make_uint2(0, 0);
+                    }
+                    counts[d][tid] = c;
+                }
+                if (C > 1) cluster_sync();
+                else __syncthreads();
+                {
+                    const int pair = tid % (kBins / 2), group = tid / (kBins / 2);
+                    uint32_t c0 = 0, c1 = 0;
+    #pragma unroll 4
+                    for (uint32_t r = group; r < C; r += kGroups) {
+                        const uint32_t c = C > 1 ? ld_cluster_u32(peer_smem(&counts[d][pair], r)) : counts[d][pair];
+                        c0 += c & 0xffffu;
+                        c1 += c >> 16;
+                    }
+                    *reinterpret_cast<uint2 *>(&sums[group][2 * pair]) = make_uint2(c0, c1);
+                }
+                __syncthreads();
+                if (warp == 0) {  // lane l has digits 255 - 8l .. 248 - 8l: a scan from the top
+                    uint32_t c[8], sum = 0;
+    #pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        c[e] = 0;
+    #pragma unroll
+                        for (int i = 0; i < kGroups; ++i) c[e] += sums[i][255 - 8 * lane - e];
+                        sum += c[e];
+                    }
+                    uint32_t above = sum;
+    #pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const uint32_t y = __shfl_up_sync(0xffffffffu, above, o);
+                        if (lane >= o) above += y;
+                    }
+                    above -= sum;
+    #pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        if (above < want && want <= above + c[e]) {
+                            found[0] = 255 - 8 * lane - e;
+                            found[1] = want - above;
+                            found[2] = c[e];
+                        }
+                        above += c[e];
+                    }
+                }
+                __syncthreads();
+                prefix = (prefix << 8) | found[0];
+                want = found[1];
+                all_from = prefix << sh;
+                if (found[2] == want) {  // all of them
+                    prefix = 0xffffffffu;
+                    break;
+                }
+                if (d == 3) ++all_from;
+            }
+        } else {
+            for (int32_t i = i0 + lane; i < i1; i += 32) keys[i] = 0;  // read below by the lane that writes it
+        }
+        // Keys from all_from on stay, and of the pages with the key `prefix` the first `want`.  What this warp's part has
         // of either:
         uint32_t n_sure = 0, n_eq = 0;
         for (int32_t i = i0 + lane; i < i1; i += 32) {
-            const uint32_t key = chosen ? keys[i] : 0;
-            const bool s = i < cand0 || i >= cand1 || key >= edge_from;
+            const uint32_t key = keys[i];
+            const bool s = i < cand0 || i >= cand1 || key >= all_from;
             n_sure += s;
-            n_eq += !s && key == edge;
+            n_eq += !s && key == prefix;
         }
         n_sure = __reduce_add_sync(0xffffffffu, n_sure);
         n_eq = __reduce_add_sync(0xffffffffu, n_eq);
@@ -326,6 +325,8 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
         eq_left = want - min(eq_before, want);  // of this slice's, the first ones
         kept_before = sure_before + min(eq_before, want);
         stay_at = sure_at + min(eq_at, eq_left);
+        edge = prefix;
+        edge_from = all_from;
     }
     // places.  The warp's list of pages that stay takes the room of its keys, behind where it reads.
     const int64_t to = (kept_before + stay_at) << p.shift;
@@ -337,7 +338,7 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
         const uint32_t below = (1u << lane) - 1;
         bool stay = i < i1;
         if (drop > 0) {
-            const uint32_t key = stay && chosen ? keys[i] : 0;
+            const uint32_t key = stay ? keys[i] : 0;
             const bool sure = stay && (i < cand0 || i >= cand1 || key >= edge_from);
             const bool eq = stay && !sure && key == edge;
             const uint32_t eqs = __ballot_sync(0xffffffffu, eq);
