@@ -119,3 +119,69 @@ def test_warps_come_together_before_the_barriers_that_ask_for_it():
             assert text[:m.start()].rstrip().endswith("__syncwarp();"), (name, m.group(0))
         assert not re.search(r"\.aligned;\\n\\t *barrier", text), name
     assert found >= 3
+
+
+# ------------------------------------------------------------------------------------------------ calls without a pause
+def test_kernels_that_start_early_read_nothing_through_the_read_only_path():
+    """A kernel that is launched behind one that still runs may not use loads for memory that never changes."""
+    csrc, found = os.path.join(ROOT, "unum_ops_b200", "csrc"), 0
+    for name in sorted(os.listdir(csrc)):
+        with open(os.path.join(csrc, name)) as f:
+            text = re.sub(r"//[^\n]*", "", f.read())
+        if name.endswith(".cu") and "wait_for_previous_kernel" in text:
+            found += 1
+            assert not re.search(r"__ldg|__restrict__|ld\.global\.nc", text), name
+    assert found == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,new", [([500, 41, 1, 177], [3, 1, 1, 100]), ([30001, 40, 300, 17771], [900, 1, 299, 5]), ([900] * 150, [1] * 150)])
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_step_of_all_operators_without_a_pause(lens, new, graph):
+    """Writes, attention that gathers weights, eviction by them and attention over what is left, launched one right behind
+    the other (every argument is as the kernels take it, so that nothing lies between), give the bits that the same calls
+    give with a pause after each.  The buffers are the same in every turn and hold other values each time."""
+    from unum_ops_b200 import append_cache, evict_cache, paged_attention
+
+    d, B, T = dev(), len(lens), sum(new)
+    q, kc, vc, table, ln = [x.to(d) for x in make_case(5, lens, 2, 16, 128, 1, "bf16", spare=1 + max(lens) % 2)]
+    W = table.shape[1]
+    assert W % 2 == 1
+    bs = torch.repeat_interleave(torch.arange(B), torch.tensor(new)).to(torch.int32).to(d)
+    pos = torch.cat([torch.arange(n - m, n) + 1 for n, m in zip(lens, new)]).to(torch.int32).to(d)
+    k, v, w = *torch.zeros(2, T, 2, 128, dtype=torch.bfloat16, device=d), torch.zeros(B, 2, W, device=d)
+
+    def step(pause):
+        append_cache(k, v, kc, vc, table, bs, pos)
+        pause()
+        a = paged_attention(q, kc, vc, table, ln, weights=w, return_lse=True)
+        pause()
+        e = evict_cache(table, ln, w, budget=33, init_pages=1, local_pages=3)
+        pause()
+        b = paged_attention(q, kc, vc, e[0], e[1], weights=e[2], return_lse=True)
+        pause()
+        return [*a, *e, *b]
+
+    start = [x.clone() for x in (kc, vc)]
+    g = torch.Generator(device=d).manual_seed(1)
+    if graph:
+        step(torch.cuda.synchronize)
+        captured = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(captured):
+            outs = step(lambda: None)
+    for turn in range(12):
+        values = [torch.randn(x.shape, generator=g, device=d).to(x.dtype) for x in (q, k, v)] + [torch.rand(w.shape, generator=g, device=d)]
+        got = []
+        for pause in (torch.cuda.synchronize, lambda: None):
+            kc.copy_(start[0]), vc.copy_(start[1])
+            for x, y in zip((q, k, v, w), values):
+                x.copy_(y)
+            torch.cuda.synchronize()
+            if graph and got:
+                captured.replay()
+                res = outs
+            else:
+                res = step(pause)
+            torch.cuda.synchronize()
+            got.append([x.clone() for x in (*res, kc, vc, w)])
+        assert all(torch.equal(x, y) for x, y in zip(*got)), turn

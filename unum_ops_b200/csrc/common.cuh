@@ -54,7 +54,10 @@ inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 
 // Programmatic dependent launch: a kernel launched with this attribute may start while the one before it in the stream
 // still runs, so that its launch is not waited for.  Such a kernel begins with wait_for_previous_kernel in every thread,
 // before it reads or writes anything and before any block ends: it returns when everything before has completed and is
-// visible, and from then on lets the kernel behind it start in the same way.
+// visible, and from then on lets the kernel behind it start in the same way.  Nothing that the kernel before may write is
+// read through the read-only path (__ldg, const __restrict__): that is for memory which does not change while a kernel runs,
+// and this one runs before those writes end; its lines are not made visible by the wait, and the compiler may move such a
+// load ahead of it.
 inline cudaLaunchAttribute behind_previous_kernel() {
     cudaLaunchAttribute a = {};
     a.id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -162,7 +162,7 @@ template <> struct Num<__half> {
 
 // ---------------------------------------------------------------------------------------------- the order of the work
 __device__ __forceinline__ int32_t length(const Params &p, int32_t b) {
-    const int32_t n = __ldg(p.lens + b);
+    const int32_t n = p.lens[b];
     return n < 0 ? 0 : (n > p.max_len ? p.max_len : n);
 }
 
@@ -549,10 +549,10 @@ __global__ void __launch_bounds__(Shape<D, MT, kNear>::kThreads, kNear ? 1 : kBl
             const uint8_t *q0 = qb + r0 * p.q_sh, *q1 = qb + (r0 + 8) * p.q_sh;
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
-                qa[k][0] = r0 < left ? __ldg(reinterpret_cast<const uint32_t *>(q0 + k * 32)) : 0u;
-                qa[k][1] = r0 + 8 < left ? __ldg(reinterpret_cast<const uint32_t *>(q1 + k * 32)) : 0u;
-                qa[k][2] = r0 < left ? __ldg(reinterpret_cast<const uint32_t *>(q0 + k * 32 + 16)) : 0u;
-                qa[k][3] = r0 + 8 < left ? __ldg(reinterpret_cast<const uint32_t *>(q1 + k * 32 + 16)) : 0u;
+                qa[k][0] = r0 < left ? *reinterpret_cast<const uint32_t *>(q0 + k * 32) : 0u;
+                qa[k][1] = r0 + 8 < left ? *reinterpret_cast<const uint32_t *>(q1 + k * 32) : 0u;
+                qa[k][2] = r0 < left ? *reinterpret_cast<const uint32_t *>(q0 + k * 32 + 16) : 0u;
+                qa[k][3] = r0 + 8 < left ? *reinterpret_cast<const uint32_t *>(q1 + k * 32 + 16) : 0u;
             }
         }
         float o[D / 8][4];

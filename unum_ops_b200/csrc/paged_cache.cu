@@ -45,9 +45,9 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
     const int64_t h = c >> p.hchunks_shift, o = (int64_t)(c & ((1 << p.hchunks_shift) - 1)) * 16;
     const int4 kv = __ldcs(reinterpret_cast<const int4 *>(p.k + t * p.k_st + h * p.k_sh + o));
     const int4 vv = __ldcs(reinterpret_cast<const int4 *>(p.v + t * p.v_st + h * p.v_sh + o));
-    const int64_t b = __ldg(p.bs + t), at = (int64_t)__ldg(p.pos + t) - 1;
+    const int64_t b = p.bs[t], at = (int64_t)p.pos[t] - 1;
     if (b < 0 || b >= p.B || at < 0 || (at >> p.shift) >= p.n_pages) return;
-    const int64_t page = __ldg(p.table + b * p.bt_stride + (at >> p.shift));
+    const int64_t page = p.table[b * p.bt_stride + (at >> p.shift)];
     const int64_t token = (page << p.shift) + (at & ((1 << p.shift) - 1));
     if (page < 0 || token >= p.n_tokens) return;
     __stcs(reinterpret_cast<int4 *>(p.kc + token * p.kc_st + h * p.kc_sh + o), kv);
@@ -117,7 +117,7 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
     const uint32_t rank = cluster_ctarank(), C = cluster_nctarank();
     const int64_t b = blockIdx.x / C;
     const int32_t P = 1 << p.shift;
-    int64_t len = __ldg(p.seqlens + b);
+    int64_t len = p.seqlens[b];
     len = len < 0 ? 0 : (len > p.n_pages * P ? p.n_pages * P : len);
     const int64_t used = (len + P - 1) >> p.shift;
     const int64_t drop = used > p.budget ? used - p.budget : 0;
@@ -144,7 +144,7 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
 
     // behind what stays: pages of the row that are not in use yet move up, and nothing fills the rest
     const int64_t me = (int64_t)rank * kEvThreads + tid, all_threads = (int64_t)C * kEvThreads;
-    for (int64_t e = used + me; e < p.n_pages; e += all_threads) nrow[e - drop] = __ldg(trow + e);
+    for (int64_t e = used + me; e < p.n_pages; e += all_threads) nrow[e - drop] = trow[e];
     for (int64_t e = me; e < drop; e += all_threads) nrow[p.n_pages - drop + e] = -1;
     for (int64_t e = drop + me; e < p.n_pages; e += all_threads) erow[e] = -1;
     const int64_t end = (used - drop) << p.shift;
@@ -185,7 +185,7 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
     #pragma unroll
                             for (int e = 0; e < kBatch; ++e)
                                 if (i00 + e * stride < n)
-                                    v[e] = __ldg(reinterpret_cast<const float4 *>(src + ((int64_t)(i00 + e * stride) << p.shift)));
+                                    v[e] = *reinterpret_cast<const float4 *>(src + ((int64_t)(i00 + e * stride) << p.shift));
     #pragma unroll
                             for (int e = 0; e < kBatch; ++e) {
                                 const int64_t left = len - ((s0 + i00 + e * stride) << p.shift) - j;
@@ -202,7 +202,7 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
     #pragma unroll
                             for (int e = 0; e < kBatch; ++e) {
                                 const int64_t at = ((int64_t)(i00 + e * stride) << p.shift);
-                                v[e] = i00 + e * stride < n && (s0 << p.shift) + at + j < len ? __ldg(src + at) : 0.0f;
+                                v[e] = i00 + e * stride < n && (s0 << p.shift) + at + j < len ? src[at] : 0.0f;
                             }
     #pragma unroll
                             for (int e = 0; e < kBatch; ++e) sum[e] += (double)v[e];
@@ -330,11 +330,11 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
     }
     // places.  The warp's list of pages that stay takes the room of its keys, behind where it reads.
     const int64_t to = (kept_before + stay_at) << p.shift;
-    int32_t m = 0, page = i0 + lane < i1 ? __ldg(trow + s0 + i0 + lane) : 0;
+    int32_t m = 0, page = i0 + lane < i1 ? trow[s0 + i0 + lane] : 0;
 #pragma unroll 1
     for (int32_t j0 = i0; j0 < i1; j0 += 32) {
         const int32_t i = j0 + lane, my_page = page;
-        if (i + 32 < i1) page = __ldg(trow + s0 + i + 32);
+        if (i + 32 < i1) page = trow[s0 + i + 32];
         const uint32_t below = (1u << lane) - 1;
         bool stay = i < i1;
         if (drop > 0) {
@@ -375,7 +375,7 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
                     float4 v[kBatch];
 #pragma unroll
                     for (int e = 0; e < kBatch; ++e)
-                        v[e] = from[e] < len ? __ldg(reinterpret_cast<const float4 *>(src + from[e]))
+                        v[e] = from[e] < len ? *reinterpret_cast<const float4 *>(src + from[e])
                                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                     for (int e = 0; e < kBatch; ++e) {
@@ -388,7 +388,7 @@ template <bool kVec> __global__ void __launch_bounds__(kEvThreads, 2) evict_kern
                 } else {
                     float v[kBatch];
 #pragma unroll
-                    for (int e = 0; e < kBatch; ++e) v[e] = from[e] < len ? __ldg(src + from[e]) : 0.0f;
+                    for (int e = 0; e < kBatch; ++e) v[e] = from[e] < len ? src[from[e]] : 0.0f;
 #pragma unroll
                     for (int e = 0; e < kBatch; ++e)
                         if (q0 + 32 * e < m) __stcs(dst + 32 * e, v[e]);
