@@ -388,8 +388,8 @@ int unum_compress_keys(const void *k, int64_t T, int64_t Hk, int64_t D, int64_t 
  *            from the caches
  *   token_to_bs, token_pos_in_bs  int32 [T]: token t is position token_pos_in_bs[t] - 1 of its sequence (the last
  *            of the positions it sees, as for unum_get_block_table)
- * A token whose sequence is outside [0, B), whose position is outside the table or whose table entry is not held
- * is not written; rows that no token goes to are left as they were.  Places must differ from token to token.
+ * A token whose sequence is outside [0, B), whose position is outside the table (or 2^31 - 2) or whose table entry
+ * is not held is not written; rows that no token goes to are left as they were.  Places must differ from token to token.
  */
 int unum_cache_append(const void *k, const void *v, int64_t T, int64_t Hk, int64_t D, int64_t k_st, int64_t k_sh,
                       int64_t v_st, int64_t v_sh, void *k_cache, void *v_cache, int64_t n_tokens, int64_t kc_st,

@@ -185,3 +185,67 @@ def test_a_step_of_all_operators_without_a_pause(lens, new, graph):
             torch.cuda.synchronize()
             got.append([x.clone() for x in (*res, kc, vc, w)])
         assert all(torch.equal(x, y) for x, y in zip(*got)), turn
+
+
+# ------------------------------------------------------------------------------------------------ ids that 32 bits do not hold
+WIDE = [(torch.int64, 1 << 32), (torch.int64, -(1 << 32)), (torch.int64, 3 << 40), (torch.uint32, 3 << 30), (torch.uint64, 1 << 63), (torch.float64, 2.0 ** 40),
+        (torch.float64, float("inf")), (torch.float32, float("nan"))]
+
+
+def widened(x, dtype, at, value):
+    """x in another type, with a value at one place."""
+    x = x.to(torch.float64 if dtype.is_floating_point else torch.int64).clone()
+    if dtype in (torch.uint32, torch.uint64):
+        x = x.clamp(min=0)
+        value = value - (1 << 64) if value >= 1 << 63 else value
+    x[at] = value
+    return x.view(dtype) if dtype == torch.uint64 else x.to(dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,value", WIDE)
+def test_ids_that_32_bits_do_not_hold(dtype, value):
+    """Wider integers and floating-point numbers are taken where int32 is asked for; what is out of its range is out of the
+    table's, the cache's and the batch's too, and a length above the bound is cut to the bound."""
+    from unum_ops_b200 import append_cache, evict_cache, paged_attention
+
+    d, lens = dev(), [40, 25]
+    q, kc, vc, table, ln = [x.to(d) for x in make_case(8, lens, 2, 4, 64, 1, "bf16")]
+    table[0, 9] = table[0, 0]
+    table[0, 0], table[0, 30:35], table[1, 25:] = 0, 1, 0
+    hidden = table.clone()
+    hidden[0, 9] = -1
+    wide = widened(table, dtype, (0, 9), value)
+    assert torch.equal(paged_attention(q, kc, vc, wide, ln), paged_attention(q, kc, vc, hidden, ln))
+    top, no_number = value > 0, value != value
+    clamped = ln.clone()
+    clamped[1] = table.shape[1] if top and not no_number else 0
+    long = widened(ln, dtype, 1, value)
+    assert torch.equal(paged_attention(q, kc, vc, table, long), paged_attention(q, kc, vc, table, clamped))
+    w = torch.rand(2, 2, table.shape[1], device=d)
+    assert all(torch.equal(x, y) for x, y in zip(evict_cache(table, long, w, budget=20), evict_cache(table, clamped, w, budget=20)))
+    k = torch.randn(3, 2, 64, device=d).to(torch.bfloat16)
+    bs, pos = torch.tensor([0, 0, 1], device=d), torch.tensor([1, 10, 3], device=d)
+    want = kc.clone()
+    want[table[0, 0].long()], want[table[1, 2].long()] = k[0], k[2]
+    for args in ((wide, bs, pos), (table, widened(bs, dtype, 1, value), pos), (table, bs, widened(pos, dtype, 1, value))):
+        a, b = kc.clone(), vc.clone()
+        append_cache(k, k, a, b, *args)
+        assert torch.equal(a, want)
+
+
+@pytest.mark.gpu
+def test_a_position_past_32_bits_in_a_table_that_reaches_so_far():
+    """A table of 2^31 positions and more: positions from 2^31 - 2 on are outside."""
+    from unum_ops_b200 import append_cache
+
+    d = dev()
+    kc, vc = torch.zeros(2, 65536, 1, 64, device=d, dtype=torch.bfloat16)
+    table = torch.full((1, 1 << 16), -1, device=d, dtype=torch.int32)
+    table[0, (1 << 15) - 1] = 0  # the page that ends at 2^31
+    k = torch.ones(3, 1, 64, device=d, dtype=torch.bfloat16)
+    pos = torch.tensor([(1 << 31) - 2, 1 << 31, 1 << 40], device=d)
+    append_cache(k, k, kc, vc, table, torch.zeros(3, dtype=torch.int32, device=d), pos, page_size=65536)
+    want = torch.zeros(65536, device=d)
+    want[65536 - 3] = 1
+    assert torch.equal(kc[:, 0, 0].float(), want) and torch.equal(vc, kc)

@@ -16,6 +16,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <string>
 #include <vector>
 
@@ -144,7 +145,19 @@ bool meet(const Tensor &a, const Tensor &b) {
     return x.first < y.second && y.first < x.second;
 }
 
-Tensor as_i32(const Tensor &t) { return (t.scalar_type() == at::kInt ? t : t.to(at::kInt)).contiguous(); }
+// Ids and lengths in the kernels' type.  What 32 bits do not hold becomes their least or largest number, which is as far
+// outside a table, a cache or a batch (a wrapped one could name another token); what is no number becomes -1.
+Tensor to_i32(const Tensor &t) {
+    const at::ScalarType type = t.scalar_type();
+    if (type == at::kInt) return t;
+    Tensor x = t;
+    if (type == at::kUInt32 || type == at::kUInt64 || at::isFloatingType(type)) x = t.to(at::kDouble).nan_to_num(-1.0);
+    if (x.scalar_type() == at::kDouble || type == at::kLong)
+        x = x.clamp(std::numeric_limits<int32_t>::min(), std::numeric_limits<int32_t>::max());
+    return x.to(at::kInt);
+}
+
+Tensor as_i32(const Tensor &t) { return to_i32(t).contiguous(); }
 
 void check_cache(const Tensor &k, const Tensor &v) {
     const char *name = "k_cache";
@@ -168,7 +181,7 @@ void check_table(const Tensor &t, int64_t page_size) {
 }
 
 Tensor table_i32(const Tensor &t) {
-    const Tensor x = t.scalar_type() == at::kInt ? t : t.to(at::kInt);
+    const Tensor x = to_i32(t);
     return x.stride(1) == 1 || x.size(1) < 2 ? x : x.contiguous();
 }
 

@@ -47,6 +47,7 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
     const int4 vv = __ldcs(reinterpret_cast<const int4 *>(p.v + t * p.v_st + h * p.v_sh + o));
     const int64_t b = p.bs[t], at = (int64_t)p.pos[t] - 1;
     if (b < 0 || b >= p.B || at < 0 || (at >> p.shift) >= p.n_pages) return;
+    if (at == INT32_MAX - 1) return;  // the largest count stands for all that 32 bits do not hold
     const int64_t page = p.table[b * p.bt_stride + (at >> p.shift)];
     const int64_t token = (page << p.shift) + (at & ((1 << p.shift) - 1));
     if (page < 0 || token >= p.n_tokens) return;

@@ -14,6 +14,10 @@ power of two, and 1 is the table that ``get_block_table`` and ``sparse_attention
 read (the same caches serve both, with ``head_group = Hk`` there).  A table entry
 outside the cache marks positions that are not held: they are neither read nor written.
 
+Tables, lengths and ids are int32; other types are converted on the way (a kernel or two
+more), and what 32 bits do not hold becomes their least or largest number: such an entry is
+outside the cache, such a length above every bound.
+
 Serving only: there is no backward pass, and inputs that ask for one are refused.
 """
 from __future__ import annotations
@@ -32,8 +36,8 @@ def append_cache(k, v, k_cache, v_cache, block_table, token_to_bs, token_pos_in_
     token_pos_in_bs  int32 [T], as for get_block_table: token t sees that many positions,
                      the last of them its own, so it is written to position
                      ``token_pos_in_bs[t] - 1``
-    A token whose sequence is outside [0, B), whose position is outside the table or whose
-    table entry is outside the cache is not written; every other row of the cache is left as
+    A token whose sequence is outside [0, B), whose position is outside the table (or 2^31 - 2
+    and more) or whose table entry is outside the cache is not written; every other row of the cache is left as
     it was.  The tokens' places must differ from each other: where two are the same, the row
     holds pieces of either.  Returns (k_cache, v_cache)."""
     _lib.binding().append_cache(k, v, k_cache, v_cache, block_table, token_to_bs, token_pos_in_bs, page_size)
