@@ -249,3 +249,51 @@ def test_a_position_past_32_bits_in_a_table_that_reaches_so_far():
     want = torch.zeros(65536, device=d)
     want[65536 - 3] = 1
     assert torch.equal(kc[:, 0, 0].float(), want) and torch.equal(vc, kc)
+
+
+# ------------------------------------------------------------------------------------------------ caches that share memory
+def cache_pairs():
+    """(k_cache, v_cache, whether they share memory) in one buffer each."""
+    D = 64
+    t = lambda *s: torch.zeros(s, dtype=torch.bfloat16)  # noqa: E731
+    b = t(13, 3, D)
+    yield b[:12], b[1:], True                                   # a token apart
+    yield b[:, :2], b[:, 1:], True                              # a head apart
+    yield b[:, :1], b[:, 1:2], False                            # heads side by side
+    yield b[:, ::2], b[:, 1:2].expand(13, 2, D)[:, :2], True    # an expanded one
+    c = t(13, 2, 2, D)
+    yield c[:, 0], c[:, 1], False                               # interleaved token by token
+    yield c[:12, 0], c[1:, 0], True
+    yield c[:12, 1], c[1:, 0], False                            # a token apart, interleaved all the same
+    yield c[:, :, 0], c[:, :, 1], False                         # interleaved head by head
+    yield c[:, :, 0], c[:, 1], True
+    yield c[:6, 0], c[7:, 0][:6], False                         # one behind the other
+    e = t(13, 6, D)
+    yield e[:, :4:2], e[:, 1:3], True                           # heads 0, 2 and 1, 2
+    yield e[:, :4:2], e[:, 1::4], False                         # heads 0, 2 and 1, 5: different strides
+    f = t(4 * 13 * D)
+    yield f[:].as_strided((13, 2, D), (4 * D, D, 1)), f.as_strided((13, 2, D), (4 * D, D, 1), D // 2), True   # half a row apart
+    yield f.as_strided((13, 2, D), (4 * D, D, 1)), f.as_strided((13, 2, D), (4 * D, D, 1), 2 * D - 8), True   # by its last piece
+    yield f.as_strided((12, 2, D), (4 * D, D, 1)), f.as_strided((12, 2, D), (4 * D, D, 1), 6 * D), False
+    yield f.as_strided((12, 2, D), (4 * D, D, 1)), f.as_strided((12, 2, D), (2 * D, D, 1), 2 * D), True       # strides of their own
+    yield t(1, 2, D), t(1, 2, D), False
+    g = t(3, D)
+    yield g[None, :2], g[None, 1:], True                        # a cache of one token
+    yield t(0, 2, D), t(0, 2, D), False
+
+
+@pytest.mark.parametrize("i", range(len(list(cache_pairs()))))
+def test_caches_that_share_memory_are_refused(i):
+    from unum_ops_b200 import append_cache
+
+    k, v, shared = list(cache_pairs())[i]
+    new, ids = torch.zeros(2, k.shape[1], 64, dtype=torch.bfloat16), torch.ones(2, dtype=torch.int32)
+    table = torch.zeros(2, 12, dtype=torch.int32)
+    for a, b in ((k, v), (v, k)):
+        with pytest.raises(ValueError, match="share memory" if shared else "CUDA"):  # these are on the CPU
+            append_cache(new, new, a, b, table, ids, ids)
+        # as the rows' addresses have it
+        rows = [{x.data_ptr() + 2 * (i * x.stride(0) + h * x.stride(1) + d) for i in range(x.shape[0]) for h in range(x.shape[1])
+                 for d in range(64)} for x in (a, b)]
+        expanded = any(len(r) < x.numel() for r, x in zip(rows, (a, b)))
+        assert shared == (expanded or bool(rows[0] & rows[1]))

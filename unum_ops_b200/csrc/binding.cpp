@@ -145,6 +145,27 @@ bool meet(const Tensor &a, const Tensor &b) {
     return x.first < y.second && y.first < x.second;
 }
 
+// Whether rows of two caches [n, Hk, D] meet; neither overlaps itself, and both have sizes and type alike.  Views that are
+// interleaved in one buffer have one token stride, and then it is a question of the heads' distances modulo that stride.
+// Interleaved with token strides of their own they count as meeting.
+bool rows_meet(const Tensor &a, const Tensor &b) {
+    if (!meet(a, b)) return false;
+    const int64_t n = a.size(0), H = a.size(1), D = a.size(2), st = stride(a, 0), sa = stride(a, 1), sb = stride(b, 1);
+    if (stride(b, 0) != st || (sa != sb && H > 256)) return true;
+    const int64_t apart = (reinterpret_cast<intptr_t>(b.const_data_ptr()) - reinterpret_cast<intptr_t>(a.const_data_ptr())) /
+                          (int64_t)a.element_size();
+    auto hit = [&](int64_t d) {  // d + i * st, |i| < n, less than a row from 0
+        int64_t i = st ? -d / st : 0;  // and its neighbours
+        for (int64_t e = std::max(i - 1, 1 - n); e <= std::min(i + 1, n - 1); ++e)
+            if (std::abs(d + e * st) < D) return true;
+        return false;
+    };
+    for (int64_t h = 0; h < H; ++h)
+        for (int64_t g = 0; g < (sa == sb && h ? 1 : H); ++g)  // with one head stride only the heads' difference counts
+            if (hit(apart + g * sb - h * sa)) return true;
+    return false;
+}
+
 // Ids and lengths in the kernels' type.  What 32 bits do not hold becomes their least or largest number, which is as far
 // outside a table, a cache or a batch (a wrapped one could name another token); what is no number becomes -1.
 Tensor to_i32(const Tensor &t) {
@@ -204,7 +225,7 @@ PyObject *append_cache(const Args &a) {
     if (k.scalar_type() != kc.scalar_type() || v.scalar_type() != kc.scalar_type())
         refuse(PyExc_ValueError, "k and v must have the cache's dtype ", kc.scalar_type(), "; got ", k.scalar_type(), " and ",
                v.scalar_type());
-    if (overlaps(kc) || overlaps(vc) || (kc.numel() && kc.const_data_ptr() == vc.const_data_ptr()))
+    if (overlaps(kc) || overlaps(vc) || rows_meet(kc, vc))
         refuse(PyExc_ValueError, "k_cache and v_cache are written to: their rows must not share memory");
     if (meet(k, kc) || meet(k, vc) || meet(v, kc) || meet(v, vc))
         refuse(PyExc_ValueError, "k and v must not lie in the memory of k_cache and v_cache");
