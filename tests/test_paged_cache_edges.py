@@ -297,3 +297,26 @@ def test_caches_that_share_memory_are_refused(i):
                  for d in range(64)} for x in (a, b)]
         expanded = any(len(r) < x.numel() for r, x in zip(rows, (a, b)))
         assert shared == (expanded or bool(rows[0] & rows[1]))
+
+
+# ------------------------------------------------------------------------------------------------ refusals
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("which", ["q", "kc", "vc", "w", "k", "v"])
+def test_tangents_are_refused(which, grad):
+    """Dual tensors of forward mode, under torch.no_grad() too, which does not turn that mode off."""
+    import torch.autograd.forward_ad as fwd
+
+    from unum_ops_b200 import append_cache, evict_cache, paged_attention
+
+    q, kc, vc, table, ln = make_case(1, [5, 9], 2, 4, 64, 1, "bf16")
+    x = dict(q=q, kc=kc, vc=vc, w=torch.zeros(2, 2, table.shape[1]), k=kc[:2].clone(), v=vc[:2].clone())
+    with fwd.dual_level(), torch.set_grad_enabled(grad):
+        x[which] = fwd.make_dual(x[which], torch.ones_like(x[which]))
+        calls = [lambda: paged_attention(x["q"], x["kc"], x["vc"], table, ln, weights=x["w"])] if which not in "kv" else []
+        if which == "w":
+            calls.append(lambda: evict_cache(table, ln, x["w"], budget=4))
+        if which not in "qw":
+            calls.append(lambda: append_cache(x["k"], x["v"], x["kc"], x["vc"], table, ln, ln))
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()

@@ -78,12 +78,18 @@ struct Args {
     bool truth(int i) const { return PyObject_IsTrue(a[i]) == 1; }
 };
 
+// Tangents of forward mode count whatever the grad mode: torch.no_grad() does not turn them off.
 void no_grad(std::initializer_list<const Tensor *> ts) {
-    if (!at::GradMode::is_enabled()) return;
-    for (const Tensor *t : ts)
-        if (t->defined() && t->requires_grad())
+    const bool backward = at::GradMode::is_enabled();
+    for (const Tensor *t : ts) {
+        if (!t->defined()) continue;
+        if (backward && t->requires_grad())
             refuse(PyExc_NotImplementedError,
                    "the paged cache's operators have no backward pass: call them under torch.no_grad()");
+        if (t->_fw_grad(/*level=*/0).defined())
+            refuse(PyExc_NotImplementedError,
+                   "the paged cache's operators have no forward-mode derivative: unpack dual tensors before the call");
+    }
 }
 
 // Called after the other checks, so that those are the same on a machine without a GPU.

@@ -18,7 +18,8 @@ Tables, lengths and ids are int32; other types are converted on the way (a kerne
 more), and what 32 bits do not hold becomes their least or largest number: such an entry is
 outside the cache, such a length above every bound.
 
-Serving only: there is no backward pass, and inputs that ask for one are refused.
+Serving only: there is no backward pass and no forward-mode derivative, and inputs that ask
+for one are refused.
 """
 from __future__ import annotations
 
