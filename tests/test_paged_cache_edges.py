@@ -320,3 +320,17 @@ def test_tangents_are_refused(which, grad):
         for call in calls:
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
+
+
+def test_a_return_lse_without_a_truth_value_raises_its_own_error():
+    from unum_ops_b200 import paged_attention
+
+    class NoTruth:
+        def __bool__(self):
+            raise ZeroDivisionError("no truth")
+
+    q, kc, vc, table, ln = make_case(1, [5, 9], 2, 4, 64, 1, "bf16")
+    with pytest.raises(ZeroDivisionError, match="no truth"):
+        paged_attention(q, kc, vc, table, ln, return_lse=NoTruth())
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        paged_attention(q, kc, vc, table, ln, return_lse=torch.zeros(2))

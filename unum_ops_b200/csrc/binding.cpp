@@ -32,6 +32,8 @@ struct Refused {
     std::string what;
 };
 
+struct Raised {};  // a Python exception that is set already
+
 std::string text(const char *s) { return s; }
 std::string text(int64_t x) { return std::to_string(x); }
 std::string text(at::ScalarType x) { return c10::toString(x); }
@@ -75,7 +77,11 @@ struct Args {
         }
         return x;
     }
-    bool truth(int i) const { return PyObject_IsTrue(a[i]) == 1; }
+    bool truth(int i) const {
+        const int x = PyObject_IsTrue(a[i]);
+        if (x < 0) throw Raised();
+        return x == 1;
+    }
 };
 
 // Tangents of forward mode count whatever the grad mode: torch.no_grad() does not turn them off.
@@ -260,6 +266,7 @@ PyObject *paged_attention(const Args &a) {
     const Tensor &table = a.tensor(3, "block_table"), &lens = a.tensor(4, "seqlens");
     const int64_t page = a.integer(5, "page_size");
     const Tensor &weights = a.optional_tensor(8, "weights");
+    const bool return_lse = a.truth(9);
     no_grad({&q, &kc, &vc, &weights});
     check_cache(kc, vc);
     if (q.dim() != 3 || q.size(2) != kc.size(2))
@@ -287,7 +294,7 @@ PyObject *paged_attention(const Args &a) {
     const c10::cuda::CUDAGuard guard(dev);
     const Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
     Tensor lse;
-    if (a.truth(9)) lse = at::empty({B, Hq}, q.options().dtype(at::kFloat));
+    if (return_lse) lse = at::empty({B, Hq}, q.options().dtype(at::kFloat));
     if (B) {
         const Tensor q_ = rows16(q), t = table_i32(table), lens_ = as_i32(lens);
         const size_t bytes = unum_paged_attention_workspace_size(B, Hq, Hk, D, max_len, weights.defined());
@@ -346,6 +353,7 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
     try {
         if (n != kArgs) refuse(PyExc_TypeError, "expected ", (int64_t)kArgs, " arguments, got ", (int64_t)n);
         return kFn(Args{args, {}});
+    } catch (const Raised &) {
     } catch (const Refused &r) {
         PyErr_SetString(r.type, r.what.c_str());
     } catch (const c10::OutOfMemoryError &e) {
