@@ -334,3 +334,22 @@ def test_a_return_lse_without_a_truth_value_raises_its_own_error():
         paged_attention(q, kc, vc, table, ln, return_lse=NoTruth())
     with pytest.raises(RuntimeError, match="ambiguous"):
         paged_attention(q, kc, vc, table, ln, return_lse=torch.zeros(2))
+
+
+# ------------------------------------------------------------------------------------------------ the build
+def test_the_binding_is_built_again_for_another_torch_or_python(monkeypatch):
+    """It is bound to torch's C++ ABI and to Python's: one compiled for others is neither current nor loaded."""
+    import sysconfig
+
+    from unum_ops_b200 import _build, _lib
+
+    _build.build()
+    assert not _build.needs_build()
+    for where, name, value in ((torch, "__version__", "2.99.0"), (sysconfig, "get_config_var", lambda _: "cpython-399")):
+        with monkeypatch.context() as m:
+            m.setattr(where, name, value)
+            assert _build.needs_build()
+            m.setattr(_lib, "_native", None)
+            with pytest.raises(RuntimeError, match="build it"):
+                _lib.binding()
+    assert not _build.needs_build()

@@ -1,12 +1,13 @@
 """Build the CUDA extension in-tree: unum_ops_b200/lib/libunum_ops_b200.so, and its
-binding to torch's tensors, unum_ops_b200/lib/_binding.so.
+binding to torch's tensors, unum_ops_b200/lib/_binding.<Python ABI>-torch<version>.so.
 
 nvcc compiles every ``csrc/*.cu`` for sm_100a only (``-gencode
 arch=compute_100a,code=sm_100a``) and links one shared library exposing the C
 ABI declared in ``include/unum_ops_b200.h``.  The CUDA runtime is linked as a
 shared library so the extension shares the runtime state (current device,
 streams) of the PyTorch process that loads it.  ``csrc/binding.cpp`` (the native
-half of ``paged_cache``) is host code against torch's headers, linked to that library.
+half of ``paged_cache``) is host code against torch's headers, linked to that library; it
+fits the torch and the Python that it was compiled for, and its file is named after them.
 
 Usage: ``python -m unum_ops_b200._build [--force]``.
 """
@@ -17,12 +18,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
+
+import torch
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(OUT_DIR, "libunum_ops_b200.so")
-BINDING = os.path.join(OUT_DIR, "_binding.so")
 ROOT = os.path.dirname(HERE)
 
 NVCC_FLAGS = [
@@ -31,6 +34,10 @@ NVCC_FLAGS = [
     "-Xptxas", "-v", "--expt-relaxed-constexpr",
     "-I" + os.path.join(ROOT, "include"),
 ]
+
+
+def binding_path() -> str:
+    return os.path.join(OUT_DIR, f"_binding.{sysconfig.get_config_var('SOABI')}-torch{torch.__version__}.so")
 
 
 def _nvcc() -> str:
@@ -48,16 +55,13 @@ def _deps():
 
 
 def needs_build() -> bool:
-    if not os.path.exists(LIB) or not os.path.exists(BINDING):
+    if not os.path.exists(LIB) or not os.path.exists(binding_path()):
         return True
-    t = min(os.path.getmtime(LIB), os.path.getmtime(BINDING))
+    t = min(os.path.getmtime(LIB), os.path.getmtime(binding_path()))
     return any(os.path.getmtime(d) > t for d in _deps())
 
 
 def _binding_command(src, out):
-    import sysconfig
-
-    import torch
     from torch.utils import cpp_extension
 
     cxx = os.environ.get("CXX") or shutil.which("g++") or "c++"
@@ -99,11 +103,11 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stderr}")
     os.replace(tmp, LIB)
-    tmp = BINDING + ".tmp"
+    tmp = binding_path() + ".tmp"
     r = subprocess.run(_binding_command(os.path.join(CSRC, "binding.cpp"), tmp), capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"binding failed:\n{r.stderr}")
-    os.replace(tmp, BINDING)
+    os.replace(tmp, binding_path())
     return LIB
 
 

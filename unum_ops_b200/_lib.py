@@ -107,7 +107,7 @@ def binding():
     global _native
     if _native is None:
         load()
-        path = _build.BINDING
+        path = _build.binding_path()
         if not os.path.exists(path):
             raise RuntimeError(f"unum_ops_b200 binding not found at {path}; build it with "
                                "`python -m unum_ops_b200._build` (there is no CPU fallback)")
