@@ -5,6 +5,8 @@ The oracles are those of test_paged_cache.py: the operators' definition in 64 bi
 """
 import os
 import re
+import threading
+import time
 
 import numpy as np
 import pytest
@@ -353,3 +355,44 @@ def test_the_binding_is_built_again_for_another_torch_or_python(monkeypatch):
             with pytest.raises(RuntimeError, match="build it"):
                 _lib.binding()
     assert not _build.needs_build()
+
+
+# ------------------------------------------------------------------------------------------------ other threads
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["append", "attend", "evict"])
+def test_other_threads_run_while_a_call_waits_for_the_device(op):
+    """A launch waits where the device's queue of launches is full (here behind a kernel that takes most of a second).
+    Python's other threads run meanwhile."""
+    from unum_ops_b200 import append_cache, evict_cache, paged_attention
+
+    q, kc, vc, table, ln = [x.to(dev()) for x in make_case(1, [5, 9], 2, 4, 64, 1, "bf16")]
+    k, w = kc[:2].clone(), torch.zeros(2, 2, table.shape[1], device=dev())
+    call = {"append": lambda: append_cache(k, k, kc, vc, table, ln, ln), "attend": lambda: paged_attention(q, kc, vc, table, ln),
+            "evict": lambda: evict_cache(table, ln, w, budget=4)}[op]
+    for _ in range(3):
+        call()
+    torch.cuda.synchronize()
+    ticks, done = [], threading.Event()
+
+    def tick():
+        while not done.is_set():
+            ticks.append(time.perf_counter())
+            time.sleep(0.002)
+
+    other = threading.Thread(target=tick)
+    other.start()
+    begin = time.perf_counter()
+    torch.cuda._sleep(1_500_000_000)
+    longest = 0.0
+    for _ in range(3000):
+        t = time.perf_counter()
+        call()
+        longest = max(longest, time.perf_counter() - t)
+    torch.cuda.synchronize()
+    end = time.perf_counter()
+    done.set()
+    other.join()
+    ticks = [begin] + [t for t in ticks if begin < t < end] + [end]
+    pause = max(b - a for a, b in zip(ticks, ticks[1:]))
+    assert longest > 0.3, "the queue never filled: nothing was tested"
+    assert pause < 0.15, (pause, longest)

@@ -15,8 +15,10 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <array>
 #include <cmath>
 #include <limits>
+#include <optional>
 #include <string>
 #include <vector>
 
@@ -222,13 +224,19 @@ void written(const Tensor &t) {  // for whoever has saved it
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// Runs f while other Python threads run: an allocation or a launch may wait for the device.  f makes no Python object.
+template <typename F> auto released(const F &f) {
+    struct Free {
+        PyThreadState *state = PyEval_SaveThread();
+        ~Free() { PyEval_RestoreThread(state); }
+    } free;
+    return f();
+}
+
 void *stream_of(c10::Device d) { return c10::cuda::getCurrentCUDAStream(d.index()).stream(); }
 
-// append_cache(k, v, k_cache, v_cache, block_table, token_to_bs, token_pos_in_bs, page_size)
-PyObject *append_cache(const Args &a) {
-    const Tensor &k = a.tensor(0, "k"), &v = a.tensor(1, "v"), &kc = a.tensor(2, "k_cache"), &vc = a.tensor(3, "v_cache");
-    const Tensor &table = a.tensor(4, "block_table"), &bs = a.tensor(5, "token_to_bs"), &pos = a.tensor(6, "token_pos_in_bs");
-    const int64_t page = a.integer(7, "page_size");
+void append(const Tensor &k, const Tensor &v, const Tensor &kc, const Tensor &vc, const Tensor &table, const Tensor &bs,
+            const Tensor &pos, int64_t page) {
     no_grad({&k, &v, &kc, &vc});
     check_cache(kc, vc);
     if (k.dim() != 3 || k.sizes() != v.sizes() || k.size(1) != kc.size(1) || k.size(2) != kc.size(2))
@@ -247,7 +255,7 @@ PyObject *append_cache(const Args &a) {
                bs.numel(), " and ", pos.numel());
     check_table(table, page);
     const c10::Device dev = on_one_gpu({&k, &v, &kc, &vc, &table, &bs, &pos});
-    if (k.numel() == 0) Py_RETURN_NONE;
+    if (k.numel() == 0) return;
     const c10::cuda::CUDAGuard guard(dev);
     const Tensor k_ = rows16(k), v_ = rows16(v), t = table_i32(table), bs_ = as_i32(bs), pos_ = as_i32(pos);
     check(unum_cache_append(k_.const_data_ptr(), v_.const_data_ptr(), T, k_.size(1), k_.size(2), stride(k_, 0), stride(k_, 1),
@@ -257,16 +265,21 @@ PyObject *append_cache(const Args &a) {
                             stream_of(dev)));
     written(kc);
     written(vc);
+}
+
+// append_cache(k, v, k_cache, v_cache, block_table, token_to_bs, token_pos_in_bs, page_size)
+PyObject *append_cache(const Args &a) {
+    const Tensor &k = a.tensor(0, "k"), &v = a.tensor(1, "v"), &kc = a.tensor(2, "k_cache"), &vc = a.tensor(3, "v_cache");
+    const Tensor &table = a.tensor(4, "block_table"), &bs = a.tensor(5, "token_to_bs"), &pos = a.tensor(6, "token_pos_in_bs");
+    const int64_t page = a.integer(7, "page_size");
+    released([&] { append(k, v, kc, vc, table, bs, pos, page); });
     Py_RETURN_NONE;
 }
 
-// paged_attention(q, k_cache, v_cache, block_table, seqlens, page_size, max_seqlen, softmax_scale, weights, return_lse)
-PyObject *paged_attention(const Args &a) {
-    const Tensor &q = a.tensor(0, "q"), &kc = a.tensor(1, "k_cache"), &vc = a.tensor(2, "v_cache");
-    const Tensor &table = a.tensor(3, "block_table"), &lens = a.tensor(4, "seqlens");
-    const int64_t page = a.integer(5, "page_size");
-    const Tensor &weights = a.optional_tensor(8, "weights");
-    const bool return_lse = a.truth(9);
+// The output and, where it is asked for, the lse.
+std::pair<Tensor, Tensor> attend(const Tensor &q, const Tensor &kc, const Tensor &vc, const Tensor &table, const Tensor &lens,
+                                 int64_t page, std::optional<int64_t> max_seqlen, std::optional<double> softmax_scale,
+                                 const Tensor &weights, bool return_lse) {
     no_grad({&q, &kc, &vc, &weights});
     check_cache(kc, vc);
     if (q.dim() != 3 || q.size(2) != kc.size(2))
@@ -281,7 +294,7 @@ PyObject *paged_attention(const Args &a) {
         refuse(PyExc_ValueError, "block_table and seqlens must have one row for each of ", B, " sequences; got ",
                table.size(0), " and ", lens.numel());
     int64_t max_len = table.size(1) * page;
-    if (a.a[6] != Py_None) max_len = std::min(max_len, a.integer(6, "max_seqlen"));
+    if (max_seqlen) max_len = std::min(max_len, *max_seqlen);
     if (max_len < 0) refuse(PyExc_ValueError, "max_seqlen must not be negative; got ", max_len);
     if (weights.defined()) {
         if (weights.dim() != 3 || weights.size(0) != B || weights.size(1) != Hk || weights.size(2) < max_len)
@@ -289,7 +302,7 @@ PyObject *paged_attention(const Args &a) {
         if (weights.scalar_type() != at::kFloat || (weights.stride(2) != 1 && weights.size(2) > 1) || overlaps(weights))
             refuse(PyExc_ValueError, "weights must be float32 with contiguous rows that share no memory");
     }
-    const double scale = a.a[7] == Py_None ? 1.0 / std::sqrt((double)D) : a.number(7, "softmax_scale");
+    const double scale = softmax_scale ? *softmax_scale : 1.0 / std::sqrt((double)D);
     const c10::Device dev = on_one_gpu({&q, &kc, &vc, &table, &lens, &weights});
     const c10::cuda::CUDAGuard guard(dev);
     const Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
@@ -309,15 +322,28 @@ PyObject *paged_attention(const Args &a) {
             weights.defined() ? weights.stride(1) : 0, ws.get(), bytes, stream_of(dev)));
         if (weights.defined()) written(weights);
     }
+    return {out, lse};
+}
+
+// paged_attention(q, k_cache, v_cache, block_table, seqlens, page_size, max_seqlen, softmax_scale, weights, return_lse)
+PyObject *paged_attention(const Args &a) {
+    const Tensor &q = a.tensor(0, "q"), &kc = a.tensor(1, "k_cache"), &vc = a.tensor(2, "v_cache");
+    const Tensor &table = a.tensor(3, "block_table"), &lens = a.tensor(4, "seqlens");
+    const int64_t page = a.integer(5, "page_size");
+    std::optional<int64_t> max_seqlen;
+    if (a.a[6] != Py_None) max_seqlen = a.integer(6, "max_seqlen");
+    std::optional<double> scale;
+    if (a.a[7] != Py_None) scale = a.number(7, "softmax_scale");
+    const Tensor &weights = a.optional_tensor(8, "weights");
+    const bool return_lse = a.truth(9);
+    const auto [out, lse] =
+        released([&] { return attend(q, kc, vc, table, lens, page, max_seqlen, scale, weights, return_lse); });
     if (!lse.defined()) return THPVariable_Wrap(out);
     return Py_BuildValue("(NN)", THPVariable_Wrap(out), THPVariable_Wrap(lse));
 }
 
-// evict_cache(block_table, seqlens, weights, budget, init_pages, local_pages, page_size)
-PyObject *evict_cache(const Args &a) {
-    const Tensor &table = a.tensor(0, "block_table"), &lens = a.tensor(1, "seqlens"), &weights = a.tensor(2, "weights");
-    const int64_t budget = a.integer(3, "budget"), init = a.integer(4, "init_pages"), local = a.integer(5, "local_pages");
-    const int64_t page = a.integer(6, "page_size");
+std::array<Tensor, 4> evict(const Tensor &table, const Tensor &lens, const Tensor &weights, int64_t budget, int64_t init,
+                            int64_t local, int64_t page) {
     no_grad({&weights});
     check_table(table, page);
     const int64_t B = table.size(0), n_pages = table.size(1);
@@ -344,8 +370,17 @@ PyObject *evict_cache(const Args &a) {
                                new_table.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(), new_w.data_ptr<float>(),
                                gone.data_ptr<int32_t>(), stream_of(dev)));
     }
-    return Py_BuildValue("(NNNN)", THPVariable_Wrap(new_table), THPVariable_Wrap(new_lens), THPVariable_Wrap(new_w),
-                         THPVariable_Wrap(gone));
+    return {new_table, new_lens, new_w, gone};
+}
+
+// evict_cache(block_table, seqlens, weights, budget, init_pages, local_pages, page_size)
+PyObject *evict_cache(const Args &a) {
+    const Tensor &table = a.tensor(0, "block_table"), &lens = a.tensor(1, "seqlens"), &weights = a.tensor(2, "weights");
+    const int64_t budget = a.integer(3, "budget"), init = a.integer(4, "init_pages"), local = a.integer(5, "local_pages");
+    const int64_t page = a.integer(6, "page_size");
+    const auto r = released([&] { return evict(table, lens, weights, budget, init, local, page); });
+    return Py_BuildValue("(NNNN)", THPVariable_Wrap(r[0]), THPVariable_Wrap(r[1]), THPVariable_Wrap(r[2]),
+                         THPVariable_Wrap(r[3]));
 }
 
 template <PyObject *(*kFn)(const Args &), int kArgs>
