@@ -5,6 +5,8 @@ The oracles are those of test_paged_cache.py: the operators' definition in 64 bi
 """
 import os
 import re
+import subprocess
+import sys
 import threading
 import time
 
@@ -396,3 +398,76 @@ def test_other_threads_run_while_a_call_waits_for_the_device(op):
     pause = max(b - a for a, b in zip(ticks, ticks[1:]))
     assert longest > 0.3, "the queue never filled: nothing was tested"
     assert pause < 0.15, (pause, longest)
+
+
+@pytest.mark.gpu
+def test_calls_from_two_threads_at_once():
+    """Each thread on a stream of its own, with sizes that take both of attention's ways."""
+    from unum_ops_b200 import append_cache, evict_cache, paged_attention
+
+    cases = []
+    for seed, lens in ((1, [700, 3, 90]), (2, [30000, 40, 17000])):
+        q, kc, vc, table, ln = [x.to(dev()) for x in make_case(seed, lens, 2, 16, 128, 1, "bf16")]
+        w = torch.rand(3, 2, table.shape[1], device=dev())
+        k = torch.randn(3, 2, 128, device=dev()).to(torch.bfloat16)
+        cases.append((q, kc, vc, table, ln, w, k, torch.arange(3, dtype=torch.int32, device=dev())))
+
+    def step(q, kc, vc, table, ln, w, k, bs):
+        w, kc, vc = w.clone(), kc.clone(), vc.clone()
+        append_cache(k, k, kc, vc, table, bs, ln)
+        out = paged_attention(q, kc, vc, table, ln, weights=w, return_lse=True)
+        with pytest.raises(ValueError, match="budget"):
+            evict_cache(table, ln, w, budget=0)
+        return [*out, *evict_cache(table, ln, w, budget=50, init_pages=2)]
+
+    want = [step(*c) for c in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(100):
+                got[i].append(step(*cases[i]))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for g, w in zip(got, want):
+        assert len(g) == 100 and all(torch.equal(x, y) for r in g for x, y in zip(r, w))
+
+
+FIRST_CALLS_IN_A_GRAPH = """
+import sys
+sys.path[:0] = [{root!r}, {tests!r}]
+import torch
+from test_paged_cache import make_case
+from unum_ops_b200 import append_cache, evict_cache, paged_attention
+for lens in ([700, 3, 90], [30000, 40, 17000]):
+    q, kc, vc, table, ln = [x.cuda() for x in make_case(1, lens, 2, 16, 128, 1, "bf16")]
+    w, k = torch.rand(3, 2, table.shape[1]).cuda(), torch.ones(3, 2, 128, dtype=torch.bfloat16).cuda()
+    bs = torch.arange(3, dtype=torch.int32).cuda()
+    start = w.clone()
+    def step():
+        append_cache(k, k, kc, vc, table, bs, ln)
+        return [*paged_attention(q, kc, vc, table, ln, weights=w, return_lse=True), *evict_cache(table, ln, w, budget=9)]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    g.replay()
+    torch.cuda.synchronize()
+    w.copy_(start)
+    assert all(torch.equal(a, b) for a, b in zip(got, step()))
+print("as they should be")
+"""
+
+
+@pytest.mark.gpu
+def test_the_first_calls_of_a_process_are_captured():
+    """What a first call sets up is allowed while a graph is captured."""
+    code = FIRST_CALLS_IN_A_GRAPH.format(root=ROOT, tests=os.path.join(ROOT, "tests"))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "as they should be" in r.stdout, r.stderr[-2000:]
