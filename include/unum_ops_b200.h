@@ -44,7 +44,8 @@ extern "C" {
 /* Message of the last failing call on this host thread ("" if none). */
 const char *unum_last_error(void);
 
-/* ABI version of this library (major * 100 + minor). */
+/* ABI version of this library (major * 100 + minor).  Entry points that are added later do not raise it: a host that may
+ * meet an older library looks for them by name. */
 int unum_abi_version(void);
 
 /*
@@ -405,7 +406,7 @@ int unum_cache_append(const void *k, const void *v, int64_t T, int64_t Hk, int64
  *   out      dtype [B, Hq, D] contiguous, fully written;  lse  float [B, Hq] or NULL
  *   weights  float [B, Hk, >= max_seqlen] or NULL (strides w_sb, w_sh): updated in place
  *   workspace  unum_paged_attention_workspace_size(...) bytes, 16-byte aligned, any contents, not shared with a
- *            call that may run at the same time
+ *            call that may run at the same time; with weights it holds B * Hq * max_seqlen scores of 4 bytes
  *
  *   s[p] = softmax_scale * q[b,h] . k[token(p), g],  g = h / G;   lse[b,h] = log sum_p exp(s[p])
  *   out[b,h] = sum_p exp(s[p] - lse) v[token(p), g];   weights[b,g,p] += sum_{h in group g} exp(s[p] - lse)

@@ -19,8 +19,9 @@
 //     copies run on across items;
 //   - the products are m16n8k16 matrix instructions with the 16 heads as rows: scores and probabilities stay in
 //     registers (the scores' layout is the layout that the second product wants), with the softmax's running maximum and
-//     sum in 32 bits; the output accumulates in registers.  Tensor memory would put a key in each of its 128 lanes and so
-//     each maximum over keys across lanes, for a product that takes 6% of the tensor cores;
+//     sum in 32 bits; the output accumulates in registers.  Tensor memory, with the keys as rows, would put a key in each
+//     of its 128 lanes and so each maximum over keys across lanes, for a product that takes 6% of the tensor cores (with
+//     the heads as rows it would not, but a tile has 64 rows at least: untried for groups of 64);
 //   - where an item is cut, each block leaves its maximum, sum and output in the workspace and a second kernel joins them
 //     in the order of the positions (the same bits each time).  It also turns the scores, left in the workspace in 32
 //     bits, into weights: their sum over the group needs each head's final lse, and reading 4 * G bytes back costs less
@@ -32,8 +33,8 @@
 // read one step ahead only, 381 + 4.8; G = 32 over 134 MB 27.5 + 5.4, G = 64 43.6 + 8.7, where the matrix instructions'
 // and the softmax's latency shows.
 // Roundings: the probabilities go to the cache's type for the product with v (the sum l uses them unrounded), and the
-// output once at the end.  The matrix instructions take no wider type beside the cache's; of an output's error against 64
-// bits, 1.7e-3 of its norm in bf16 and 2.1e-4 in fp16 with the last rounding alone, the two make 2.4e-3 and 2.7e-4.
+// output once at the end.  The matrix instructions take no wider type beside the cache's; an output's error against 64
+// bits, 1.7e-3 of its norm in bf16 and 2.0e-4 in fp16 with the last rounding alone, is 2.3e-3 and 2.6e-4 with both.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -11,8 +11,9 @@
 //
 // evict: of each sequence's pages in use the first `init`, the last `local` and the heaviest others stay, `budget`
 //   in all.  A page's weight is the sum over kv heads and the page's positions of the weights that paged attention
-//   gathered, taken in 64 bits and rounded to 32 once, so that no order of summation decides which page stays; ties
-//   go to the lower index and a NaN ranks below every number.  The row closes up over what is evicted.
+//   gathered, taken in 64 bits and rounded to 32 once: another order of summation gives another weight only where the
+//   sum lies within a few 2^-53 of its terms from a border of the rounding.  Ties go to the lower index and a NaN ranks
+//   below every number.  The row closes up over what is evicted.
 #include <cuda_runtime.h>
 
 #include "common.cuh"

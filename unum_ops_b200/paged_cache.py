@@ -55,7 +55,8 @@ def paged_attention(q, k_cache, v_cache, block_table, seqlens, *, page_size=1, m
                  among them, once ``append_cache`` has written it); counts outside
                  [0, max_seqlen] are clamped
     max_seqlen   an upper bound of seqlens known on the host (default: what the table
-                 holds): sizes the launch and, with ``weights``, its workspace
+                 holds): sizes the launch and, with ``weights``, its workspace of
+                 B * Hq * max_seqlen * 4 bytes
     weights      float32 [B, Hk, W >= max_seqlen], updated in place: weights[b, g, p] grows by
                  the softmax weights that the group's G heads give position p; positions
                  that are not attended to keep their value.  ``evict_cache`` reads them
@@ -78,7 +79,8 @@ def evict_cache(block_table, seqlens, weights, *, budget, init_pages=0, local_pa
     last ``local_pages`` (at least one) and the heaviest others stay, ``budget`` in all, in
     their order; a sequence that has no more than that keeps them all.  A page's weight is the
     sum of its positions' weights over all kv heads, in 64 bits and rounded to 32 once; ties
-    stay by the lower index and a NaN ranks below every number.
+    stay by the lower index and a NaN ranks below every number.  With ``budget ==
+    init_pages + local_pages`` nothing is chosen, and the weights only move along.
     Returns new tensors (block_table, seqlens, weights, evicted):
         block_table  the rows without the evicted pages (entries behind the pages in use move up
                      too), -1 at the end
