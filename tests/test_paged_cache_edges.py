@@ -191,6 +191,58 @@ def test_a_step_of_all_operators_without_a_pause(lens, new, graph):
         assert all(torch.equal(x, y) for x, y in zip(*got)), turn
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[500, 41, 0, 177], [30000, 40, 300, 17771]])
+@pytest.mark.parametrize("graph", [False, True])
+def test_two_streams_that_part_and_meet(lens, graph):
+    """Copies into the inputs, a write, attention on two streams at once, and eviction on the first by what the other has
+    gathered: eager, and as one graph with a fork and a join."""
+    from unum_ops_b200 import append_cache, evict_cache, paged_attention
+
+    d = dev()
+    q, kc, vc, table, ln = [x.to(d) for x in make_case(6, lens, 2, 16, 128, 1, "bf16")]
+    W = table.shape[1]
+    qs, qs_in, ws = [torch.empty_like(q) for _ in range(2)], [torch.empty_like(q) for _ in range(2)], [torch.zeros(4, 2, W, device=d) for _ in range(2)]
+    k, bs = torch.randn(4, 2, 128, device=d).to(torch.bfloat16), torch.arange(4, dtype=torch.int32, device=d)
+    side, g = torch.cuda.Stream(), torch.Generator(device=d).manual_seed(3)
+
+    def step(other):
+        for x, y, w in zip(qs, qs_in, ws):
+            x.copy_(y)
+            w.zero_()
+        append_cache(k, k, kc, vc, table, bs, ln)
+        main = torch.cuda.current_stream()
+        if other:
+            other.wait_stream(main)
+        with torch.cuda.stream(other or main):
+            a = paged_attention(qs[0], kc, vc, table, ln, weights=ws[0], return_lse=True)
+        b = paged_attention(qs[1], kc, vc, table, ln, weights=ws[1], return_lse=True)
+        if other:
+            main.wait_stream(other)
+        e = evict_cache(table, ln, ws[0], budget=30)
+        c = paged_attention(qs[0], kc, vc, e[0], e[1], weights=ws[1], return_lse=True)
+        return [*a, *b, *e, *c, *ws]
+
+    if graph:
+        step(None)
+        torch.cuda.synchronize()
+        captured = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(captured):
+            outs = step(side)
+    for _ in range(10):
+        for x in qs_in:
+            x.copy_(torch.randn(x.shape, generator=g, device=d))
+        torch.cuda.synchronize()
+        want = [x.clone() for x in step(None)]
+        torch.cuda.synchronize()
+        if graph:
+            captured.replay()
+        else:
+            outs = step(side)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(outs, want))
+
+
 # ------------------------------------------------------------------------------------------------ ids that 32 bits do not hold
 WIDE = [(torch.int64, 1 << 32), (torch.int64, -(1 << 32)), (torch.int64, 3 << 40), (torch.uint32, 3 << 30), (torch.uint64, 1 << 63), (torch.float64, 2.0 ** 40),
         (torch.float64, float("inf")), (torch.float32, float("nan"))]
@@ -397,7 +449,7 @@ def test_other_threads_run_while_a_call_waits_for_the_device(op):
     ticks = [begin] + [t for t in ticks if begin < t < end] + [end]
     pause = max(b - a for a, b in zip(ticks, ticks[1:]))
     assert longest > 0.3, "the queue never filled: nothing was tested"
-    assert pause < 0.15, (pause, longest)
+    assert pause < longest / 2, (pause, longest)
 
 
 @pytest.mark.gpu
