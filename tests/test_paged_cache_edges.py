@@ -135,7 +135,7 @@ def test_kernels_that_start_early_read_nothing_through_the_read_only_path():
         if name.endswith(".cu") and "wait_for_previous_kernel" in text:
             found += 1
             assert not re.search(r"__ldg|__restrict__|ld\.global\.nc", text), name
-    assert found == 2
+    assert found >= 2
 
 
 @pytest.mark.gpu
